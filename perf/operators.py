@@ -361,7 +361,7 @@ def _plain_plan(s):
     # who is let in: the table has room, then the row buffers, then the stack
     new = asked.clamp(min=0)
     fits = ~ends & (length + new <= stride * page)
-    fits &= torch.where(fits, new, 0).cumsum(0) <= capacity
+    fits &= (new == 0) | (torch.where(fits, new, 0).cumsum(0) <= capacity)
     need = torch.where(fits, (length + new + page - 1) // page - held, 0)
     before = need.cumsum(0) - need
     fits &= (need == 0) | (before + need <= stack)
