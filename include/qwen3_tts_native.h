@@ -496,6 +496,149 @@ QWEN3_TTS_API int32_t qwen3_tts_op_sum_embeddings(
     int32_t width, const int32_t* tokens, uint16_t* output, void* stream, char* error,
     size_t error_capacity);
 
+/* Paged 8-bit key/value cache of many sequences (no counterpart in the
+ * reference, whose sessions reserve one contiguous bf16 cache each).  A step
+ * of a server is one kv8_plan, then per layer one kv8_append and one
+ * kv8_attention; none of the three allocates, synchronises or reads back, so
+ * a step can be captured into a HIP graph.  All pointers are device memory of
+ * the current device, on which `stream` lies.
+ *
+ * A page holds page_tokens tokens of every key/value head as 8-bit values, one
+ * array of pages for keys and one for values, with one fp32 scale per page and
+ * head: a value is held * scale.  Per head a page is a run of 2048-byte
+ * granules of 16 tokens; token t (0..15), dimension d of a granule lies at byte
+ *   keys:   (d / 64) * 1024 + t * 64 + d % 64
+ *   values: (d / 64) * 1024 + (t / 4) * 256 + (d % 16) * 16 + (d / 16 % 4) * 4 + t % 4 */
+enum {
+    QWEN3_TTS_KV8_INT8 = 0, /* -127..127 */
+    QWEN3_TTS_KV8_E4M3 = 1, /* OCP e4m3 (no infinities), up to 448 */
+};
+typedef struct Qwen3TtsKv8CacheV1 {
+    uint32_t struct_size;
+    int32_t format;
+    int32_t page_tokens;     /* 16, 32 or 64 */
+    int32_t pages;           /* pages * page_tokens < 2^31 */
+    int32_t key_value_heads;
+    int32_t head_dimension;  /* 128 */
+    uint8_t* key_pages;      /* [pages][key_value_heads][page_tokens / 16][2048], 16-byte aligned */
+    uint8_t* value_pages;
+    float* key_scales;       /* [pages][key_value_heads] */
+    float* value_scales;
+} Qwen3TtsKv8CacheV1;
+
+/* Block tables, row map and slots of a step, from the sequences' lengths.
+ * Sequence s holds lengths[s] tokens in the pages tables[s][0 ..] and asks for
+ * new_tokens[s] more:
+ *   < 0: it ends.  Its pages go on the stack free_pages[0 .. free_count), in
+ *        the table's order, sequences in theirs; its new length is 0.
+ *   >= 0: it is let in if its table has room; then, unless it brings no rows,
+ *        if its rows and those of all earlier sequences that passed so far
+ *        fit rows_capacity; then, unless it needs no page, if its pages and
+ *        those that the earlier ones that passed so far need lie on the
+ *        stack (pages given back in this call included).  Page j
+ *        comes from below those of the sequences before it, from the top.
+ *        One that is not let in keeps its length, gets no rows and counts in
+ *        *refused.
+ * Rows of the sequences follow one another: row_starts[s] .. row_starts[s+1]
+ * are those of sequence s (sequences + 1 entries); row r gets its position
+ * and its slot page * page_tokens + position % page_tokens.  Rows behind the
+ * last one, up to rows_capacity, get slot -1 and position 0, so that a graph
+ * with a fixed number of rows can append and attend with fewer.
+ * new_lengths may be lengths and new_free_count may be free_count; other
+ * buffers must not overlap.  A page may stand in several tables (a shared
+ * prefix) while no sequence writes to it or ends: giving back a page twice
+ * puts it on the stack twice. */
+typedef struct Qwen3TtsKv8PlanV1 {
+    uint32_t struct_size;
+    int32_t sequences;
+    int32_t page_tokens;     /* 16, 32 or 64 */
+    int32_t pages;           /* of the cache: entries of free_pages */
+    int32_t table_stride;    /* entries of a sequence in tables */
+    int32_t rows_capacity;   /* entries of row_positions and row_slots */
+    const int32_t* new_tokens;   /* [sequences] */
+    const int32_t* lengths;      /* [sequences] */
+    int32_t* new_lengths;        /* [sequences] */
+    int32_t* tables;             /* [sequences][table_stride] */
+    int32_t* free_pages;         /* [pages] */
+    const int32_t* free_count;   /* [1] */
+    int32_t* new_free_count;     /* [1] */
+    int32_t* row_starts;         /* [sequences + 1] */
+    int32_t* row_positions;      /* [rows_capacity] */
+    int32_t* row_slots;          /* [rows_capacity] */
+    int32_t* refused;            /* [1] */
+} Qwen3TtsKv8PlanV1;
+QWEN3_TTS_API int32_t qwen3_tts_op_kv8_plan_v1(
+    const Qwen3TtsKv8PlanV1* args, void* stream, char* error, size_t error_capacity);
+
+/* Stores bf16 key and value rows [rows][stride] (key_value_heads * 128 values
+ * each; strides in elements, multiples of 8; 16-byte aligned) at their slots.
+ * A slot outside the cache, -1 for instance, leaves its row out.  Slots of one
+ * page have to follow one another in one run of rising slots, as the plan makes
+ * them (a page that is met in two runs of one call gets undefined contents);
+ * tokens of the page behind the run no longer count.  Scale of a page and head,
+ * keys and values apart: the largest finite magnitude of the run / 127 (int8)
+ * or the smallest power of two whose 448-fold is no smaller (e4m3), and never
+ * less than the page's scale where the run does not begin the page; earlier
+ * tokens are then rounded anew to the larger scale.  Values are rounded to
+ * nearest even; infinities become the largest held value, NaN becomes 0. */
+typedef struct Qwen3TtsKv8AppendV1 {
+    uint32_t struct_size;
+    int32_t rows;
+    int32_t key_stride;
+    int32_t value_stride;
+    const uint16_t* key;
+    const uint16_t* value;
+    const int32_t* row_slots;    /* [rows] */
+} Qwen3TtsKv8AppendV1;
+QWEN3_TTS_API int32_t qwen3_tts_op_kv8_append_v1(
+    const Qwen3TtsKv8CacheV1* cache, const Qwen3TtsKv8AppendV1* args, void* stream, char* error,
+    size_t error_capacity);
+
+/* Causal attention of rows of many sequences, prompts and single tokens
+ * together: row i of sequence s (rows row_starts[s] .. row_starts[s+1], the last
+ * ones of its lengths[s] tokens) attends to its own position and those before
+ * it, the last `window` of them where window > 0.  Scores are scale * q.k;
+ * query head h reads key/value head h / (query_heads / key_value_heads), at
+ * most 16 of them share one.  Rows that no sequence has are left as they were; a row
+ * with nothing to attend to becomes 0, and a table entry that is no page
+ * counts as nothing.  query and out are bf16 [rows][stride] (strides in
+ * elements, multiples of 8 and 4; 16- and 8-byte aligned) and may be the same.
+ * max_rows and max_length are what the caller knows of the largest sequence's
+ * rows and length (the graph's, where it is captured): they choose how the work is
+ * dealt out, results hold beyond them.  workspace is scratch for sharing long
+ * contexts among workgroups, 16-byte aligned; what the size query names is
+ * used where it is given, less works too, and none.  Calls that may run at
+ * the same time need workspaces of their own. */
+typedef struct Qwen3TtsKv8AttentionV1 {
+    uint32_t struct_size;
+    int32_t query_heads;
+    int32_t rows;
+    int32_t query_stride;
+    int32_t out_stride;
+    int32_t sequences;           /* up to 65535 */
+    int32_t table_stride;
+    int32_t max_rows;
+    int32_t max_length;
+    int32_t window;
+    float scale;
+    int32_t reserved;            /* 0 */
+    const uint16_t* query;
+    uint16_t* out;
+    const int32_t* tables;       /* [sequences][table_stride] */
+    const int32_t* lengths;      /* [sequences], the step's own rows included */
+    const int32_t* row_starts;   /* [sequences + 1] */
+    void* workspace;
+    uint64_t workspace_bytes;
+} Qwen3TtsKv8AttentionV1;
+QWEN3_TTS_API int32_t qwen3_tts_op_kv8_attention_v1(
+    const Qwen3TtsKv8CacheV1* cache, const Qwen3TtsKv8AttentionV1* args, void* stream, char* error,
+    size_t error_capacity);
+/* Bytes of workspace that a call with these sizes uses (pointers and
+ * workspace_bytes are not looked at). */
+QWEN3_TTS_API int32_t qwen3_tts_op_kv8_attention_workspace_v1(
+    const Qwen3TtsKv8CacheV1* cache, const Qwen3TtsKv8AttentionV1* args, uint64_t* bytes, char* error,
+    size_t error_capacity);
+
 /* Device memory / stream helpers for harnesses. */
 QWEN3_TTS_API int32_t qwen3_tts_device_malloc(int32_t device_index, uint64_t bytes, void** output,
                                               char* error, size_t error_capacity);

@@ -7,6 +7,7 @@
 // runtime.cu (probe :86-122, argmax benchmark :124-255), gemv.cu:88-270,
 // primitive_parity.cu:115-368 and weights.cu:1-340.
 #include "q3_common.hpp"
+#include "kv8.hpp"
 
 #include "../../include/qwen3_tts_native.h"
 
@@ -66,6 +67,52 @@ int32_t launch_status(hipError_t status, const char* what, char* error, size_t c
 }
 
 hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
+
+// Arguments of the kv8 ops as the launchers take them; a message where a
+// struct is missing or of another size.
+const char* kv8_cache_of(const Qwen3TtsKv8CacheV1* c, Kv8Cache& out) {
+    if (c == nullptr || c->struct_size != sizeof(*c)) return "cache is null or has an unsupported size";
+    if (c->head_dimension != kKv8HeadDimension) return "head_dimension must be 128";
+    out.format = c->format;
+    out.page_tokens = c->page_tokens;
+    out.pages = c->pages;
+    out.key_value_heads = c->key_value_heads;
+    out.key_pages = c->key_pages;
+    out.value_pages = c->value_pages;
+    out.key_scales = c->key_scales;
+    out.value_scales = c->value_scales;
+    return nullptr;
+}
+
+const char* kv8_attention_of(const Qwen3TtsKv8AttentionV1* a, Kv8AttentionArgs& out) {
+    if (a == nullptr || a->struct_size != sizeof(*a)) return "arguments are null or have an unsupported size";
+    if (a->reserved != 0) return "reserved must be 0";
+    out.query_heads = a->query_heads;
+    out.rows = a->rows;
+    out.query_stride = a->query_stride;
+    out.out_stride = a->out_stride;
+    out.sequences = a->sequences;
+    out.table_stride = a->table_stride;
+    out.max_rows = a->max_rows;
+    out.max_length = a->max_length;
+    out.window = a->window;
+    out.scale = a->scale;
+    out.query = a->query;
+    out.out = a->out;
+    out.tables = a->tables;
+    out.lengths = a->lengths;
+    out.row_starts = a->row_starts;
+    out.workspace = static_cast<float*>(a->workspace);
+    out.workspace_bytes = a->workspace_bytes;
+    return nullptr;
+}
+
+int32_t invalid(const char* what, const char* why, char* error, size_t capacity) {
+    char message[256];
+    std::snprintf(message, sizeof(message), "%s: %s", what, why);
+    write_error(error, capacity, message);
+    return QWEN3_TTS_TALKER_STATUS_INVALID_ARGUMENT;
+}
 
 constexpr int kWarmupIterations = 20;
 
@@ -817,6 +864,73 @@ QWEN3_TTS_API int32_t qwen3_tts_op_sum_embeddings(const uint16_t* const* tables,
                                                   uint16_t* output, void* stream, char* error, size_t cap) {
     return launch_status(launch_sum_embeddings(tables, count, vocabulary0, vocabulary, width, tokens, output, as_stream(stream)),
                          "sum embeddings", error, cap);
+}
+
+// ---------------------------------------------------------------------------
+// Paged 8-bit key/value cache
+// ---------------------------------------------------------------------------
+QWEN3_TTS_API int32_t qwen3_tts_op_kv8_plan_v1(const Qwen3TtsKv8PlanV1* args, void* stream, char* error, size_t cap) {
+    if (args == nullptr || args->struct_size != sizeof(*args)) {
+        return invalid("kv8 plan", "arguments are null or have an unsupported size", error, cap);
+    }
+    Kv8PlanArgs p;
+    p.sequences = args->sequences;
+    p.page_tokens = args->page_tokens;
+    p.pages = args->pages;
+    p.table_stride = args->table_stride;
+    p.rows_capacity = args->rows_capacity;
+    p.new_tokens = args->new_tokens;
+    p.lengths = args->lengths;
+    p.new_lengths = args->new_lengths;
+    p.tables = args->tables;
+    p.free_pages = args->free_pages;
+    p.free_count = args->free_count;
+    p.new_free_count = args->new_free_count;
+    p.row_starts = args->row_starts;
+    p.row_positions = args->row_positions;
+    p.row_slots = args->row_slots;
+    p.refused = args->refused;
+    return launch_status(launch_kv8_plan(p, as_stream(stream)), "kv8 plan", error, cap);
+}
+
+QWEN3_TTS_API int32_t qwen3_tts_op_kv8_append_v1(const Qwen3TtsKv8CacheV1* cache, const Qwen3TtsKv8AppendV1* args,
+                                                 void* stream, char* error, size_t cap) {
+    Kv8Cache c;
+    if (const char* why = kv8_cache_of(cache, c)) return invalid("kv8 append", why, error, cap);
+    if (args == nullptr || args->struct_size != sizeof(*args)) {
+        return invalid("kv8 append", "arguments are null or have an unsupported size", error, cap);
+    }
+    Kv8AppendArgs a;
+    a.rows = args->rows;
+    a.key_stride = args->key_stride;
+    a.value_stride = args->value_stride;
+    a.key = args->key;
+    a.value = args->value;
+    a.row_slots = args->row_slots;
+    return launch_status(launch_kv8_append(c, a, as_stream(stream)), "kv8 append", error, cap);
+}
+
+QWEN3_TTS_API int32_t qwen3_tts_op_kv8_attention_v1(const Qwen3TtsKv8CacheV1* cache, const Qwen3TtsKv8AttentionV1* args,
+                                                    void* stream, char* error, size_t cap) {
+    Kv8Cache c;
+    if (const char* why = kv8_cache_of(cache, c)) return invalid("kv8 attention", why, error, cap);
+    Kv8AttentionArgs a;
+    if (const char* why = kv8_attention_of(args, a)) return invalid("kv8 attention", why, error, cap);
+    return launch_status(launch_kv8_attention(c, a, as_stream(stream)), "kv8 attention", error, cap);
+}
+
+QWEN3_TTS_API int32_t qwen3_tts_op_kv8_attention_workspace_v1(const Qwen3TtsKv8CacheV1* cache,
+                                                              const Qwen3TtsKv8AttentionV1* args, uint64_t* bytes,
+                                                              char* error, size_t cap) {
+    Kv8Cache c;
+    if (const char* why = kv8_cache_of(cache, c)) return invalid("kv8 attention workspace", why, error, cap);
+    Kv8AttentionArgs a;
+    if (const char* why = kv8_attention_of(args, a)) return invalid("kv8 attention workspace", why, error, cap);
+    if (bytes == nullptr) return invalid("kv8 attention workspace", "output is null", error, cap);
+    size_t need = 0;
+    const hipError_t st = kv8_attention_workspace(c, a, need);
+    if (st == hipSuccess) *bytes = need;
+    return launch_status(st, "kv8 attention workspace", error, cap);
 }
 
 QWEN3_TTS_API int32_t qwen3_tts_device_malloc(int32_t device_index, uint64_t bytes, void** output, char* error,

@@ -141,6 +141,39 @@ class StepBenchmarkV1(C.Structure):
         ("gemv_kernel_milliseconds_per_step", C.c_double), ("output_checksum", C.c_uint64)]
 
 
+KV8_INT8, KV8_E4M3 = 0, 1
+KV8_FORMATS = {"int8": KV8_INT8, "e4m3": KV8_E4M3}
+
+
+class Kv8CacheV1(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("format", C.c_int32), ("page_tokens", C.c_int32),
+                ("pages", C.c_int32), ("key_value_heads", C.c_int32), ("head_dimension", C.c_int32),
+                ("key_pages", C.c_void_p), ("value_pages", C.c_void_p), ("key_scales", C.c_void_p),
+                ("value_scales", C.c_void_p)]
+
+
+class Kv8PlanV1(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32)] + [
+        (n, C.c_int32) for n in ("sequences", "page_tokens", "pages", "table_stride", "rows_capacity")] + [
+        (n, C.c_void_p) for n in (
+            "new_tokens", "lengths", "new_lengths", "tables", "free_pages", "free_count", "new_free_count",
+            "row_starts", "row_positions", "row_slots", "refused")]
+
+
+class Kv8AppendV1(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("rows", C.c_int32), ("key_stride", C.c_int32),
+                ("value_stride", C.c_int32), ("key", C.c_void_p), ("value", C.c_void_p), ("row_slots", C.c_void_p)]
+
+
+class Kv8AttentionV1(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32)] + [
+        (n, C.c_int32) for n in ("query_heads", "rows", "query_stride", "out_stride", "sequences", "table_stride",
+                                 "max_rows", "max_length", "window")] + [
+        ("scale", C.c_float), ("reserved", C.c_int32)] + [
+        (n, C.c_void_p) for n in ("query", "out", "tables", "lengths", "row_starts", "workspace")] + [
+        ("workspace_bytes", C.c_uint64)]
+
+
 # Layouts pinned by the reference's Rust FFI test (native_talker.rs:1734-1744).
 ABI_SIZES = {
     SamplingConfig: 20, PrefillResult: 12, CodecFrameInfo: 16, ModelMemory: 16,
@@ -216,6 +249,11 @@ SIGNATURES = {
     "qwen3_tts_op_elementwise": (I32, [I32, P, P, I32, I32, P] + ERR),
     "qwen3_tts_op_sample_logits": (I32, [P, I32, I32, I32, P, P, SamplingConfig, P, P, P] + ERR),
     "qwen3_tts_op_sum_embeddings": (I32, [P, I32, I32, I32, I32, P, P, P] + ERR),
+    "qwen3_tts_op_kv8_plan_v1": (I32, [C.POINTER(Kv8PlanV1), P] + ERR),
+    "qwen3_tts_op_kv8_append_v1": (I32, [C.POINTER(Kv8CacheV1), C.POINTER(Kv8AppendV1), P] + ERR),
+    "qwen3_tts_op_kv8_attention_v1": (I32, [C.POINTER(Kv8CacheV1), C.POINTER(Kv8AttentionV1), P] + ERR),
+    "qwen3_tts_op_kv8_attention_workspace_v1": (I32, [C.POINTER(Kv8CacheV1), C.POINTER(Kv8AttentionV1),
+                                                      C.POINTER(U64)] + ERR),
     "qwen3_tts_device_malloc": (I32, [I32, U64, C.POINTER(P)] + ERR),
     "qwen3_tts_device_free": (None, [P]),
     "qwen3_tts_device_memcpy": (I32, [P, P, U64] + ERR),
@@ -353,6 +391,72 @@ def quantize_weight_rows(weight: DeviceArray, quantized: DeviceArray, scales: De
                          in_features: int, out_features: int) -> None:
     call("qwen3_tts_quantize_weight_rows_v1", weight.ptr, quantized.ptr, scales.ptr,
          in_features, out_features, None)
+
+
+# ---------------------------------------------------------------------------
+# Paged 8-bit key/value cache (include/qwen3_tts_native.h, Qwen3TtsKv8*).
+# Arrays are DeviceArrays, torch tensors on the device, or addresses.
+# ---------------------------------------------------------------------------
+def _address(array) -> int | None:
+    if array is None or isinstance(array, int):
+        return array
+    pointer = getattr(array, "data_ptr", None)
+    return pointer() if pointer is not None else array.ptr
+
+
+class Kv8Cache:
+    """A layer's pages and scales; `format` is "int8" or "e4m3"."""
+
+    def __init__(self, format: str, page_tokens: int, pages: int, key_value_heads: int, key_pages, value_pages,
+                 key_scales, value_scales):
+        self.arrays = (key_pages, value_pages, key_scales, value_scales)
+        self.key_value_heads = key_value_heads
+        self.struct = Kv8CacheV1(C.sizeof(Kv8CacheV1), KV8_FORMATS[format], page_tokens, pages, key_value_heads, 128,
+                                 *map(_address, self.arrays))
+
+
+def kv8_plan(sequences: int, page_tokens: int, pages: int, tables, table_stride: int, new_tokens, lengths, new_lengths,
+             free_pages, free_count, new_free_count, row_starts, row_positions, row_slots, rows_capacity: int, refused,
+             *, stream: int | None = None) -> None:
+    """Gives out pages and makes the row map of one step."""
+    a = Kv8PlanV1(C.sizeof(Kv8PlanV1), sequences, page_tokens, pages, table_stride, rows_capacity,
+                  _address(new_tokens), _address(lengths), _address(new_lengths), _address(tables),
+                  _address(free_pages), _address(free_count), _address(new_free_count), _address(row_starts),
+                  _address(row_positions), _address(row_slots), _address(refused))
+    call("qwen3_tts_op_kv8_plan_v1", C.byref(a), stream)
+
+
+def kv8_append(cache: Kv8Cache, key, value, row_slots, rows: int, *, key_stride: int | None = None,
+               value_stride: int | None = None, stream: int | None = None) -> None:
+    """Stores bf16 key and value rows at their slots (strides in elements)."""
+    width = cache.key_value_heads * 128
+    a = Kv8AppendV1(C.sizeof(Kv8AppendV1), rows, width if key_stride is None else key_stride,
+                    width if value_stride is None else value_stride, _address(key), _address(value),
+                    _address(row_slots))
+    call("qwen3_tts_op_kv8_append_v1", C.byref(cache.struct), C.byref(a), stream)
+
+
+def kv8_attention(cache: Kv8Cache, query, out, query_heads: int, rows: int, sequences: int, tables, table_stride: int,
+                  lengths, row_starts, *, scale: float = 128 ** -0.5, window: int = 0, max_rows: int, max_length: int,
+                  query_stride: int | None = None, out_stride: int | None = None, workspace=None,
+                  workspace_bytes: int = 0, stream: int | None = None) -> None:
+    """Causal attention of the step's query rows over their sequences' pages."""
+    width = query_heads * 128
+    a = Kv8AttentionV1(C.sizeof(Kv8AttentionV1), query_heads, rows, width if query_stride is None else query_stride,
+                       width if out_stride is None else out_stride, sequences, table_stride, max_rows, max_length,
+                       window, scale, 0, _address(query), _address(out), _address(tables), _address(lengths),
+                       _address(row_starts), _address(workspace), workspace_bytes)
+    call("qwen3_tts_op_kv8_attention_v1", C.byref(cache.struct), C.byref(a), stream)
+
+
+def kv8_attention_workspace(cache: Kv8Cache, query_heads: int, rows: int, sequences: int, *, window: int = 0,
+                            max_rows: int, max_length: int) -> int:
+    """Bytes of workspace that kv8_attention uses for these sizes."""
+    a = Kv8AttentionV1(struct_size=C.sizeof(Kv8AttentionV1), query_heads=query_heads, rows=rows, sequences=sequences,
+                       max_rows=max_rows, max_length=max_length, window=window)
+    size = U64()
+    call("qwen3_tts_op_kv8_attention_workspace_v1", C.byref(cache.struct), C.byref(a), C.byref(size))
+    return size.value
 
 
 def sampling(do_sample=0, top_k=0, top_p=1.0, temperature=1.0, repetition_penalty=1.0) -> SamplingConfig:
