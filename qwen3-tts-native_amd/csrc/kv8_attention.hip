@@ -11,6 +11,7 @@
 // accumulators are fp32.
 #include "kv8.hpp"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -29,8 +30,9 @@ struct Params {
     Kv8Cache cache;
     int group = 1;     // query heads of a key/value head
     float scale2 = 0;  // scale * log2(e)
-    int splits = 1;    // workgroups that share a context
-    int columns = 16;  // of a partial result: (row, head of the group) pairs
+    int splits = 1;    // workgroups that share a context of few rows
+    int columns = 16;  // (row, head of the group) pairs that a shared context can have
+    int few = INT_MAX;  // pairs up to which a sequence counts as one of few rows
     float* partial_out = nullptr;   // [sequence][kv head][column][split][128]
     float2* partial_sums = nullptr;  // [sequence][kv head][column][split] (maximum, sum)
 };
@@ -52,6 +54,17 @@ __device__ __forceinline__ Rows rows_of(const Params& p, int sequence) {
     return r;
 }
 
+// Workgroups that share the context of a sequence of few rows: 0 where it is
+// not one, 1 where its results do not fit the partial ones' place (more rows
+// than the caller said).
+__device__ __forceinline__ int splits_of(const Params& p, const Rows& r) {
+    if (r.count <= 0 || r.count > p.few / p.group) return 0;
+    return r.count <= p.columns / p.group ? p.splits : 1;
+}
+__device__ __forceinline__ size_t partial_slot(const Params& p, int sequence, int kv_head, int column) {
+    return ((static_cast<size_t>(sequence) * p.cache.key_value_heads + kv_head) * p.columns + column) * p.splits;
+}
+
 // ---------------------------------------------------------------------------
 // Few rows: up to 16 (row, head) pairs of one key/value head are the columns
 // of 16x16x32 products, keys and values are read once for all of them.
@@ -67,9 +80,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
     constexpr int kPage = kPageGranules * kKv8Granule;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int column = lane & 15, quad = lane >> 4;
-    const int split = blockIdx.x, kv_head = blockIdx.y, sequence = blockIdx.z;
+    const int kv_head = blockIdx.x, split = blockIdx.y, sequence = blockIdx.z;
     const Rows rows = rows_of(p, sequence);
-    if (rows.count <= 0) return;
+    const int splits = splits_of(p, rows);
+    if (split >= splits) return;
     const int rows_per_tile = 16 / p.group;
     const int head = kv_head * p.group + column % p.group;
     const int* table = p.a.tables + static_cast<size_t>(sequence) * p.a.table_stride;
@@ -102,7 +116,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
         const int end = min(rows.position + last + 1, rows.length);
         const int begin = p.a.window > 0 ? max(rows.position + tile - p.a.window + 1, 0) & ~(kStep - 1) : 0;
         const int steps = end > begin ? (end - begin + kStep - 1) / kStep : 0;
-        const int share = (steps + p.splits - 1) / p.splits;
+        const int share = (steps + splits - 1) / splits;
         const int steps_begin = split * share, steps_end = min(steps_begin + share, steps);
         const int lowest = p.a.window > 0 ? position - p.a.window : -1;  // tokens above it count
 
@@ -218,14 +232,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
         __syncthreads();
         // wave w: dimensions 32 w .. 32 w + 31 (two tiles of 16) of every column
         if (mine) {
-            const size_t slot = ((static_cast<size_t>(sequence) * p.cache.key_value_heads + kv_head) * p.columns + tile * p.group + column) * p.splits + split;
+            const size_t slot = partial_slot(p, sequence, kv_head, column) + split;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int d = 2 * wave + j;
                 floatx4_t o = *reinterpret_cast<const floatx4_t*>(&out_lds[0][(d * 64 + lane) * 4]);
 #pragma unroll
                 for (int w = 1; w < kWaves; ++w) o += *reinterpret_cast<const floatx4_t*>(&out_lds[w][(d * 64 + lane) * 4]);
-                if (p.splits == 1) {
+                if (splits == 1) {
                     const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
                     bf16_t* to = p.a.out + static_cast<size_t>(rows.first + row) * p.a.out_stride + head * kDim + 16 * d + 4 * quad;
                     *reinterpret_cast<uint2*>(to) = uint2{pack_bf16(o[0] * inverse, o[1] * inverse), pack_bf16(o[2] * inverse, o[3] * inverse)};
@@ -233,21 +247,313 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
                     *reinterpret_cast<floatx4_t*>(p.partial_out + slot * kDim + 16 * d + 4 * quad) = o;
                 }
             }
-            if (p.splits > 1 && wave == 0 && quad == 0) p.partial_sums[slot] = float2{top, total};
+            if (splits > 1 && wave == 0 && quad == 0) p.partial_sums[slot] = float2{top, total};
         }
         __syncthreads();
     }
 }
 
-template <int kFormat>
-hipError_t launch_few_rows(const Params& p, hipStream_t stream) {
-    const dim3 grid(p.splits, p.cache.key_value_heads, p.a.sequences);
-    switch (p.cache.page_tokens) {
-        case 16: kv8_few_rows_kernel<kFormat, 1><<<grid, 64 * kWaves, 0, stream>>>(p); break;
-        case 32: kv8_few_rows_kernel<kFormat, 2><<<grid, 64 * kWaves, 0, stream>>>(p); break;
-        default: kv8_few_rows_kernel<kFormat, 4><<<grid, 64 * kWaves, 0, stream>>>(p); break;
+// Joins the results of workgroups that shared a context: a wave a (row, head).
+__global__ __launch_bounds__(64 * kWaves) void kv8_join_kernel(Params p) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kv_head = blockIdx.x, sequence = blockIdx.y;
+    const Rows rows = rows_of(p, sequence);
+    const int splits = splits_of(p, rows);
+    if (splits <= 1) return;
+    for (int column = wave; column < rows.count * p.group; column += kWaves) {
+        const size_t slot = partial_slot(p, sequence, kv_head, column);
+        float top = -INFINITY;
+        for (int i = lane; i < splits; i += 64) top = fmaxf(top, p.partial_sums[slot + i].x);
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        const float reference = top == -INFINITY ? 0.0f : top;
+        float total = 0.0f;
+        floatx2_t o{0.f, 0.f};
+        for (int i = 0; i < splits; ++i) {
+            const float2 part = p.partial_sums[slot + i];
+            const float share = __builtin_amdgcn_exp2f(part.x - reference);
+            total += part.y * share;
+            o += *reinterpret_cast<const floatx2_t*>(p.partial_out + (slot + i) * kDim + 2 * lane) * share;
+        }
+        const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
+        const int row = rows.first + column / p.group, head = kv_head * p.group + column % p.group;
+        *reinterpret_cast<unsigned*>(p.a.out + static_cast<size_t>(row) * p.a.out_stride + head * kDim + 2 * lane) =
+            pack_bf16(o[0] * inverse, o[1] * inverse);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: a wave owns 32 (row, head) pairs of a key/value head as the
+// columns of 32x32x16 products, the block's waves share its keys and values,
+// which go through LDS as bf16: a byte is converted once for all columns.
+// Scores are formed transposed, S^T = K Q^T, with key rows dealt so that a
+// lane's scores are those of eight consecutive tokens, the operand of the value
+// product O^T = V^T P^T: weights never leave their lane.
+// ---------------------------------------------------------------------------
+constexpr int kTile = 64;  // tokens in LDS at a time
+constexpr int kTileGranules = kTile / kKv8Granule;
+// a maximum may stay this far (log2) behind the scores before the sums are scaled anew
+constexpr float kSlack = 8.0f;
+
+template <int kFormat, int kPageGranules, int kManyWaves>
+__global__ __launch_bounds__(64 * kManyWaves, 2) void kv8_many_rows_kernel(Params p) {
+    static_assert(kManyWaves == kTileGranules, "a wave stages a granule");
+    __shared__ __align__(16) unsigned char key_lds[2][kTile * kDim * 2];    // [token][16-byte groups of dimensions, swizzled]
+    __shared__ __align__(16) unsigned char value_lds[2][kTile * kDim * 2];  // [dimension][16-byte groups of tokens, swizzled]
+    __shared__ float key_scale_lds[2][kTileGranules], value_scale_lds[2][kTileGranules];
+    __shared__ int held_lds[2][kTileGranules];
+    constexpr int kPage = kPageGranules * kKv8Granule;
+    constexpr int kColumns = 32 * kManyWaves;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int column = lane & 31, half = lane >> 5;
+    const int kv_head = blockIdx.x, sequence = blockIdx.z;
+    const Rows rows = rows_of(p, sequence);
+    if (rows.count <= 0 || splits_of(p, rows) > 0) return;
+    const int* table = p.a.tables + static_cast<size_t>(sequence) * p.a.table_stride;
+    const size_t page_bytes = static_cast<size_t>(p.cache.key_value_heads) * (kPageGranules * kKv8GranuleBytes);
+    const unsigned char* keys = p.cache.key_pages + kv_head * (kPageGranules * kKv8GranuleBytes) + lane * 16;
+    const unsigned char* values = p.cache.value_pages + kv_head * (kPageGranules * kKv8GranuleBytes) + lane * 16;
+    const int pairs = rows.count * p.group;
+    const int tiles = (pairs + kColumns - 1) / kColumns;
+
+    // the longest rows first: they are the launch's tail
+    for (int tile = tiles - 1 - static_cast<int>(blockIdx.y); tile >= 0; tile -= gridDim.y) {
+        const int pair = tile * kColumns + wave * 32 + column;
+        const bool mine = pair < pairs;
+        const int row = min(pair, pairs - 1) / p.group;
+        const int head = kv_head * p.group + pair % p.group;
+        const int position = rows.position + row;
+        const int lowest = p.a.window > 0 ? position - p.a.window : -1;  // tokens above it count
+        bf16x8_t q[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            uint4 w{0, 0, 0, 0};
+            if (mine) {
+                w = *reinterpret_cast<const uint4*>(p.a.query + static_cast<size_t>(rows.first + row) * p.a.query_stride +
+                                                    head * kDim + 16 * k + 8 * half);
+            }
+            q[k] = __builtin_bit_cast(bf16x8_t, w);
+        }
+        // the block's and the wave's positions
+        const int first_row = tile * kColumns / p.group;
+        const int last_row = min(tile * kColumns + kColumns - 1, pairs - 1) / p.group;
+        const int end = min(rows.position + last_row + 1, rows.length);
+        const int begin = p.a.window > 0 ? max(rows.position + first_row - p.a.window + 1, 0) & ~(kTile - 1) : 0;
+        const int steps = end > begin ? (end - begin + kTile - 1) / kTile : 0;
+        const int wave_pair = tile * kColumns + wave * 32;
+        const bool wave_lives = wave_pair < pairs;
+        const int wave_first = rows.position + min(wave_pair, pairs - 1) / p.group;
+        const int wave_last = rows.position + min(wave_pair + 31, pairs - 1) / p.group;
+
+        uint4 k_bytes[2], v_bytes[2];
+        float key_scale = 0.f, value_scale = 0.f;
+        int held = 0;
+        auto load = [&](int step) {
+            const int first = begin + step * kTile + wave * kKv8Granule;
+            const int at = min(first, (end - 1) & ~(kKv8Granule - 1));
+            int page = table[at / kPage];
+            held = min(max(end - first, 0), kKv8Granule);
+            if (page < 0 || page >= p.cache.pages) page = 0, held = 0;
+            const size_t offset = page * page_bytes + at % kPage / kKv8Granule * kKv8GranuleBytes;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                k_bytes[c] = *reinterpret_cast<const uint4*>(keys + offset + c * 1024);
+                v_bytes[c] = *reinterpret_cast<const uint4*>(values + offset + c * 1024);
+            }
+            const size_t scale_at = static_cast<size_t>(page) * p.cache.key_value_heads + kv_head;
+            key_scale = p.cache.key_scales[scale_at] * p.scale2;
+            value_scale = p.cache.value_scales[scale_at];
+        };
+        auto stage = [&](int buffer) {
+            // keys: lane (token, 16-dimension group): two 16-byte groups of bf16 for each half of the dimensions
+            const int token = wave * kKv8Granule + (lane >> 2);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const uint2 a = bf16_of<kFormat>(k_bytes[c].x), b = bf16_of<kFormat>(k_bytes[c].y);
+                const uint2 d = bf16_of<kFormat>(k_bytes[c].z), e = bf16_of<kFormat>(k_bytes[c].w);
+                const int group = 8 * c + 2 * (lane & 3);
+                *reinterpret_cast<uint4*>(&key_lds[buffer][token * 256 + (group ^ (token & 15)) * 16]) = uint4{a.x, a.y, b.x, b.y};
+                *reinterpret_cast<uint4*>(&key_lds[buffer][token * 256 + ((group + 1) ^ (token & 15)) * 16]) = uint4{d.x, d.y, e.x, e.y};
+            }
+            // values: lane (token / 4, d % 16): four tokens of dimensions 64 c + 16 t + d % 16
+            const unsigned mask = byte_mask(4 * (lane >> 4), 0, held);
+            const int place = 2 * wave + (lane >> 5);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const unsigned w[4] = {v_bytes[c].x, v_bytes[c].y, v_bytes[c].z, v_bytes[c].w};
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int d = 64 * c + 16 * t + (lane & 15);
+                    *reinterpret_cast<uint2*>(&value_lds[buffer][d * 128 + (place ^ (d >> 1 & 7)) * 16 + (lane >> 4 & 1) * 8]) =
+                        bf16_of<kFormat>(w[t] & mask);
+                }
+            }
+            if (lane == 0) {
+                key_scale_lds[buffer][wave] = held > 0 ? key_scale : 0.0f;
+                value_scale_lds[buffer][wave] = held > 0 ? value_scale : 0.0f;
+                held_lds[buffer][wave] = held;
+            }
+        };
+
+        float maximum = -INFINITY, sum = 0.0f;
+        floatx16_t acc[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+        if (steps > 0) load(0);
+        for (int step = 0; step < steps; ++step) {
+            const int buffer = step & 1;
+            stage(buffer);
+            if (step + 1 < steps) load(step + 1);
+            __syncthreads();
+            const int token0 = begin + step * kTile;
+            if (!wave_lives || token0 > wave_last || (p.a.window > 0 && token0 + kTile - 1 <= wave_first - p.a.window)) continue;
+            // row i of a 32-token tile is token i with bits 2 and 3 exchanged
+            const int token = (column & 19) | (column & 4) << 1 | (column & 8) >> 1;
+            floatx16_t s[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+                const unsigned char* from = &key_lds[buffer][(32 * t + token) * 256];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(from + ((2 * k + half) ^ (token & 15)) * 16);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[k], s[t], 0, 0, 0);
+                }
+            }
+            float factor[kTileGranules], value_factor[kTileGranules];
+            bool whole = token0 + kTile - 1 <= wave_first && (p.a.window == 0 || token0 > wave_last - p.a.window);
+#pragma unroll
+            for (int g = 0; g < kTileGranules; ++g) {
+                factor[g] = key_scale_lds[buffer][g];
+                value_factor[g] = value_scale_lds[buffer][g];
+                whole &= held_lds[buffer][g] == kKv8Granule;
+            }
+            // s[t][i]: token 32 t + 16 (i / 8) + 8 half + i % 8
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] *= factor[2 * t + (i >> 3)];
+            if (!__builtin_amdgcn_readfirstlane(whole)) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int of_granule = 8 * half + (i & 7);
+                        const int at = token0 + 32 * t + 16 * (i >> 3) + of_granule;
+                        const bool counts = at <= position && at > lowest && of_granule < held_lds[buffer][2 * t + (i >> 3)];
+                        s[t][i] = counts ? s[t][i] : -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            if (__any(top > maximum + kSlack)) {
+                const float next = fmaxf(maximum, top);
+                const float shrink = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(maximum - next);
+                maximum = next;
+                sum *= shrink;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
+            }
+            const float reference = maximum == -INFINITY ? 0.0f : maximum;
+            bf16x8_t weights[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                unsigned w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = __builtin_amdgcn_exp2f(s[g >> 1][8 * (g & 1) + 2 * i] - reference);
+                    const float b = __builtin_amdgcn_exp2f(s[g >> 1][8 * (g & 1) + 2 * i + 1] - reference);
+                    sum += a + b;
+                    w[i] = pack_bf16(a * value_factor[g], b * value_factor[g]);
+                }
+                weights[g] = __builtin_bit_cast(bf16x8_t, uint4{w[0], w[1], w[2], w[3]});
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const int dimension = 32 * d + column;
+                const unsigned char* from = &value_lds[buffer][dimension * 128];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(from + ((2 * g + half) ^ (dimension >> 1 & 7)) * 16);
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, weights[g], acc[d], 0, 0, 0);
+                }
+            }
+        }
+        __syncthreads();  // the next tile of rows stages into the buffers
+        sum += __shfl_xor(sum, 32, 64);
+        if (mine) {
+            const float inverse = sum > 0.0f ? 1.0f / sum : 0.0f;
+            bf16_t* to = p.a.out + static_cast<size_t>(rows.first + row) * p.a.out_stride + head * kDim + 4 * half;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    *reinterpret_cast<uint2*>(to + 32 * d + 8 * i) =
+                        uint2{pack_bf16(acc[d][4 * i] * inverse, acc[d][4 * i + 1] * inverse),
+                              pack_bf16(acc[d][4 * i + 2] * inverse, acc[d][4 * i + 3] * inverse)};
+                }
+        }
+    }
+}
+
+template <int kFormat, int kPageGranules>
+hipError_t launch_pages(const Params& p, hipStream_t stream) {
+    const bool many = p.few != INT_MAX;
+    if (!many || p.a.sequences > 1) {
+        kv8_few_rows_kernel<kFormat, kPageGranules>
+            <<<dim3(p.cache.key_value_heads, p.splits, p.a.sequences), 64 * kWaves, 0, stream>>>(p);
+        if (p.splits > 1) {
+            kv8_join_kernel<<<dim3(p.cache.key_value_heads, p.a.sequences), 64 * kWaves, 0, stream>>>(p);
+        }
+    }
+    if (many) {
+        const int pairs = std::min(p.a.max_rows, p.a.rows) * p.group;
+        const int tiles = (pairs + 127) / 128;
+        kv8_many_rows_kernel<kFormat, kPageGranules, 4>
+            <<<dim3(p.cache.key_value_heads, std::min(tiles, 65535), p.a.sequences), 256, 0, stream>>>(p);
     }
     return hipGetLastError();
+}
+
+template <int kFormat>
+hipError_t launch_format(const Params& p, hipStream_t stream) {
+    switch (p.cache.page_tokens) {
+        case 16: return launch_pages<kFormat, 1>(p, stream);
+        case 32: return launch_pages<kFormat, 2>(p, stream);
+        default: return launch_pages<kFormat, 4>(p, stream);
+    }
+}
+
+// How a call's work is dealt out.
+struct Dealt {
+    bool many;    // sequences of many rows may be among them
+    int columns;  // as in Params
+    int splits;
+};
+constexpr int kBytesOfPartial = (kDim + 2) * 4;
+Dealt dealt_of(const Kv8Cache& cache, const Kv8AttentionArgs& a, size_t workspace_bytes) {
+    Dealt d;
+    const int group = a.query_heads / cache.key_value_heads;
+    const int rows = std::max(1, std::min(a.max_rows, a.rows));
+    d.many = static_cast<long long>(rows) * group > 16;
+    d.columns = std::min(16 / group, rows) * group;
+    // Contexts are shared until two workgroups a CU are there, each with a step for every wave
+    const long long blocks = static_cast<long long>(std::max(a.sequences, 1)) * cache.key_value_heads;
+    const int reach = a.window > 0 ? std::min(a.window + rows, a.max_length) : a.max_length;
+    const long long wanted = std::min<long long>((512 + blocks - 1) / blocks, (reach + kWaves * kStep - 1) / (kWaves * kStep));
+    const long long fits = static_cast<long long>(workspace_bytes / (static_cast<size_t>(blocks) * d.columns * kBytesOfPartial));
+    d.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({wanted, fits, 64})));
+    if (d.many && a.sequences == 1) d.splits = 1;  // one prompt: no sequence of few rows
+    return d;
 }
 
 bool sizes_ok(const Kv8Cache& c, const Kv8AttentionArgs& a) {
@@ -269,7 +575,8 @@ bool args_ok(const Kv8Cache& c, const Kv8AttentionArgs& a) {
 
 hipError_t kv8_attention_workspace(const Kv8Cache& cache, const Kv8AttentionArgs& a, size_t& bytes) {
     if (!sizes_ok(cache, a)) return hipErrorInvalidValue;
-    bytes = 0;
+    const Dealt d = dealt_of(cache, a, SIZE_MAX);
+    bytes = d.splits == 1 ? 0 : static_cast<size_t>(a.sequences) * cache.key_value_heads * d.columns * d.splits * kBytesOfPartial;
     return hipSuccess;
 }
 
@@ -282,7 +589,14 @@ hipError_t launch_kv8_attention(const Kv8Cache& cache, const Kv8AttentionArgs& a
     p.cache = cache;
     p.group = a.query_heads / cache.key_value_heads;
     p.scale2 = a.scale * kLog2E;
-    return cache.format == kKv8Int8 ? launch_few_rows<kKv8Int8>(p, stream) : launch_few_rows<kKv8E4m3>(p, stream);
+    const Dealt d = dealt_of(cache, a, a.workspace_bytes);
+    p.columns = d.columns;
+    p.splits = d.splits;
+    p.few = !d.many ? INT_MAX : a.sequences > 1 ? 16 : 0;
+    const size_t slots = static_cast<size_t>(a.sequences) * cache.key_value_heads * d.columns * d.splits;
+    p.partial_out = a.workspace;
+    p.partial_sums = reinterpret_cast<float2*>(a.workspace + slots * kDim);
+    return cache.format == kKv8Int8 ? launch_format<kKv8Int8>(p, stream) : launch_format<kKv8E4m3>(p, stream);
 }
 
 }  // namespace q3
