@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import pathlib
+import threading
 
 import numpy as np
 
@@ -288,11 +289,20 @@ def load(path: os.PathLike | str | None = None) -> C.CDLL:
     return lib
 
 
+class _ErrorBuffer(threading.local):
+    """A thread's buffer for the library's messages: one for all of its calls."""
+
+    def __init__(self):
+        self.text = C.create_string_buffer(512)
+
+
+_ERROR = _ErrorBuffer()
+
+
 def call(name: str, *args) -> None:
     """Invoke a status-returning export and raise Qwen3TtsError on failure."""
-    lib = load()
-    err = C.create_string_buffer(512)
-    status = getattr(lib, name)(*args, err, C.sizeof(err))
+    err = _ERROR.text
+    status = getattr(_LIB or load(), name)(*args, err, 512)
     if status != STATUS_OK:
         raise Qwen3TtsError(status, err.value.decode(errors="replace"))
 
@@ -398,10 +408,13 @@ def quantize_weight_rows(weight: DeviceArray, quantized: DeviceArray, scales: De
 # Arrays are DeviceArrays, torch tensors on the device, or addresses.
 # ---------------------------------------------------------------------------
 def _address(array) -> int | None:
-    if array is None or isinstance(array, int):
-        return array
-    pointer = getattr(array, "data_ptr", None)
-    return pointer() if pointer is not None else array.ptr
+    if hasattr(array, "data_ptr"):
+        return array.data_ptr()
+    return array if array is None or isinstance(array, int) else array.ptr
+
+
+_KV8_CACHE_BYTES, _KV8_PLAN_BYTES = C.sizeof(Kv8CacheV1), C.sizeof(Kv8PlanV1)
+_KV8_APPEND_BYTES, _KV8_ATTENTION_BYTES = C.sizeof(Kv8AppendV1), C.sizeof(Kv8AttentionV1)
 
 
 class Kv8Cache:
@@ -411,7 +424,7 @@ class Kv8Cache:
                  key_scales, value_scales):
         self.arrays = (key_pages, value_pages, key_scales, value_scales)
         self.key_value_heads = key_value_heads
-        self.struct = Kv8CacheV1(C.sizeof(Kv8CacheV1), KV8_FORMATS[format], page_tokens, pages, key_value_heads, 128,
+        self.struct = Kv8CacheV1(_KV8_CACHE_BYTES, KV8_FORMATS[format], page_tokens, pages, key_value_heads, 128,
                                  *map(_address, self.arrays))
 
 
@@ -419,21 +432,21 @@ def kv8_plan(sequences: int, page_tokens: int, pages: int, tables, table_stride:
              free_pages, free_count, new_free_count, row_starts, row_positions, row_slots, rows_capacity: int, refused,
              *, stream: int | None = None) -> None:
     """Gives out pages and makes the row map of one step."""
-    a = Kv8PlanV1(C.sizeof(Kv8PlanV1), sequences, page_tokens, pages, table_stride, rows_capacity,
+    a = Kv8PlanV1(_KV8_PLAN_BYTES, sequences, page_tokens, pages, table_stride, rows_capacity,
                   _address(new_tokens), _address(lengths), _address(new_lengths), _address(tables),
                   _address(free_pages), _address(free_count), _address(new_free_count), _address(row_starts),
                   _address(row_positions), _address(row_slots), _address(refused))
-    call("qwen3_tts_op_kv8_plan_v1", C.byref(a), stream)
+    call("qwen3_tts_op_kv8_plan_v1", a, stream)
 
 
 def kv8_append(cache: Kv8Cache, key, value, row_slots, rows: int, *, key_stride: int | None = None,
                value_stride: int | None = None, stream: int | None = None) -> None:
     """Stores bf16 key and value rows at their slots (strides in elements)."""
     width = cache.key_value_heads * 128
-    a = Kv8AppendV1(C.sizeof(Kv8AppendV1), rows, width if key_stride is None else key_stride,
+    a = Kv8AppendV1(_KV8_APPEND_BYTES, rows, width if key_stride is None else key_stride,
                     width if value_stride is None else value_stride, _address(key), _address(value),
                     _address(row_slots))
-    call("qwen3_tts_op_kv8_append_v1", C.byref(cache.struct), C.byref(a), stream)
+    call("qwen3_tts_op_kv8_append_v1", cache.struct, a, stream)
 
 
 def kv8_attention(cache: Kv8Cache, query, out, query_heads: int, rows: int, sequences: int, tables, table_stride: int,
@@ -442,17 +455,17 @@ def kv8_attention(cache: Kv8Cache, query, out, query_heads: int, rows: int, sequ
                   workspace_bytes: int = 0, stream: int | None = None) -> None:
     """Causal attention of the step's query rows over their sequences' pages."""
     width = query_heads * 128
-    a = Kv8AttentionV1(C.sizeof(Kv8AttentionV1), query_heads, rows, width if query_stride is None else query_stride,
+    a = Kv8AttentionV1(_KV8_ATTENTION_BYTES, query_heads, rows, width if query_stride is None else query_stride,
                        width if out_stride is None else out_stride, sequences, table_stride, max_rows, max_length,
                        window, scale, 0, _address(query), _address(out), _address(tables), _address(lengths),
                        _address(row_starts), _address(workspace), workspace_bytes)
-    call("qwen3_tts_op_kv8_attention_v1", C.byref(cache.struct), C.byref(a), stream)
+    call("qwen3_tts_op_kv8_attention_v1", cache.struct, a, stream)
 
 
 def kv8_attention_workspace(cache: Kv8Cache, query_heads: int, rows: int, sequences: int, *, window: int = 0,
                             max_rows: int, max_length: int) -> int:
     """Bytes of workspace that kv8_attention uses for these sizes."""
-    a = Kv8AttentionV1(struct_size=C.sizeof(Kv8AttentionV1), query_heads=query_heads, rows=rows, sequences=sequences,
+    a = Kv8AttentionV1(struct_size=_KV8_ATTENTION_BYTES, query_heads=query_heads, rows=rows, sequences=sequences,
                        max_rows=max_rows, max_length=max_length, window=window)
     size = U64()
     call("qwen3_tts_op_kv8_attention_workspace_v1", C.byref(cache.struct), C.byref(a), C.byref(size))

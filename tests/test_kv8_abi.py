@@ -69,7 +69,7 @@ def test_bad_caches_are_refused(hip, changes):
 
 @pytest.mark.parametrize("changes", [
     dict(struct_size=0), dict(sequences=0), dict(sequences=-1), dict(page_tokens=17), dict(pages=0),
-    dict(pages=1 << 28), dict(table_stride=0), dict(table_stride=1 << 28), dict(rows_capacity=-1), dict(lengths=None),
+    dict(pages=1 << 28), dict(table_stride=0), dict(table_stride=1 << 28), dict(rows_capacity=-1), dict(rows_capacity=1 << 30), dict(lengths=None),
     dict(new_tokens=None), dict(new_lengths=None), dict(tables=None), dict(free_pages=None), dict(free_count=None),
     dict(new_free_count=None), dict(row_starts=None), dict(row_positions=None), dict(row_slots=None),
     dict(refused=None), dict(lengths=FAKE + 1)])
