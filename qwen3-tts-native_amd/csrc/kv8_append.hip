@@ -18,13 +18,17 @@
 // with the run and keep their bytes where it does not: nothing reads them
 // before a later run writes them.
 //
-// A wave owns a (run, head, keys or values): nobody else touches the page's
-// bytes of that head, so granules that the run enters half-way are read,
-// merged and written whole.  Lane (token, 16-dimension group) quantises in the
-// keys' layout; values take their layout through 2 KB of LDS.  Bound by HBM for
-// prompts, by the chain slot -> scale and page -> store for single tokens.
+// A workgroup owns a (run, head, keys or values), a wave each granule of the
+// page: nobody else touches the page's bytes of that head, so granules that
+// the run enters half-way are read, merged and written whole.  Lane (token,
+// 16-dimension group) quantises in the keys' layout; values take theirs by two
+// 4 x 4 transpositions in registers, of bytes over the lanes of four tokens
+// and of words over the four lane groups.  Bound by HBM for prompts (16379 rows,
+// 8 heads, int8: 4.2 TB/s), by the chain slot -> page and scale -> store for
+// single tokens.
 #include "kv8.hpp"
 
+#include <algorithm>
 #include <climits>
 
 namespace q3 {
@@ -32,21 +36,26 @@ namespace {
 
 using namespace kv8;
 
-// Bytes of four values from their quotients x / S.
+constexpr int kRows = 64;  // rows that a workgroup looks at for runs
+
+// Bytes of four values from their quotients x / S.  Adding 1.5 * 2^52 rounds to
+// the nearest whole number, ties to even, and leaves it in the low bits.
 template <int kFormat>
 __device__ __forceinline__ unsigned hold4(double a, double b, double c, double d) {
     if constexpr (kFormat == kKv8Int8) {
-        // NaN passes neither bound: fmax returns the bound, so it is caught by the callers
-        const auto one = [](double v) { return static_cast<unsigned>(static_cast<int>(fmin(fmax(rint(v), -127.0), 127.0))) & 0xffu; };
-        return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+        const auto one = [](double v) {
+            return static_cast<unsigned>(__builtin_bit_cast(unsigned long long, v + 6755399441055744.0));
+        };
+        const unsigned low = __builtin_amdgcn_perm(one(b), one(a), 0x0c0c0400u);
+        return __builtin_amdgcn_perm(one(d), one(c), 0x04000c0cu) | low;
     } else {
         const auto one = [](double v) { return fminf(fmaxf(static_cast<float>(v), -448.0f), 448.0f); };
-        int w = __builtin_amdgcn_cvt_pk_fp8_f32(one(a), one(b), 0, false);
+        const int w = __builtin_amdgcn_cvt_pk_fp8_f32(one(a), one(b), 0, false);
         return static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(one(c), one(d), w, true));
     }
 }
 
-// Held values in a page whose scale changed by `ratio` = S_old / S.
+// Held values in a page whose scale changed by `ratio` = S_old / S, at most 1.
 template <int kFormat>
 __device__ __forceinline__ unsigned rescale4(unsigned w, double ratio) {
     if constexpr (kFormat == kKv8Int8) {
@@ -58,6 +67,11 @@ __device__ __forceinline__ unsigned rescale4(unsigned w, double ratio) {
         return hold4<kFormat>(at(__builtin_amdgcn_cvt_f32_fp8(w, 0)), at(__builtin_amdgcn_cvt_f32_fp8(w, 1)),
                               at(__builtin_amdgcn_cvt_f32_fp8(w, 2)), at(__builtin_amdgcn_cvt_f32_fp8(w, 3)));
     }
+}
+template <int kFormat>
+__device__ __forceinline__ uint4 rescale16(uint4 w, double ratio) {
+    return uint4{rescale4<kFormat>(w.x, ratio), rescale4<kFormat>(w.y, ratio), rescale4<kFormat>(w.z, ratio),
+                 rescale4<kFormat>(w.w, ratio)};
 }
 
 template <int kFormat>
@@ -73,167 +87,188 @@ __device__ __forceinline__ float scale_for(float largest) {
     }
 }
 
-__device__ __forceinline__ int wave_max(int v) {
+template <int kControl>
+__device__ __forceinline__ unsigned max_moved(unsigned v) {
+    return max(v, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kControl, 0xf, 0xf, true)));
+}
+
+// The largest value over the workgroup's waves.
+template <int kWaves>
+__device__ __forceinline__ unsigned block_max(unsigned v, unsigned* lds) {
+    v = max(v, static_cast<unsigned>(__builtin_amdgcn_permlane32_swap(v, v, false, false)[1]));  // lanes 0-31 see 32-63
+    v = max(v, static_cast<unsigned>(__builtin_amdgcn_permlane16_swap(v, v, false, false)[1]));  // lanes 0-15 see 16-31
+    v = max_moved<0x108>(v);  // row_shl:8 and below
+    v = max_moved<0x104>(v);
+    v = max_moved<0x102>(v);
+    v = max_moved<0x101>(v);
+    v = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
+    if constexpr (kWaves == 1) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v = max(v, __shfl_xor(v, d, 64));
+    for (int w = 1; w < kWaves; ++w) v = max(v, lds[w]);
     return v;
 }
 
+// Of the four lanes 4 n .. 4 n + 3, lane k gets byte k of each one's word.
+__device__ __forceinline__ unsigned transpose_bytes(unsigned w, int lane) {
+    const unsigned next = static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w), 0xb1, 0xf, 0xf, true));  // lane ^ 1
+    w = __builtin_amdgcn_perm(next, w, lane & 1 ? 0x03070105u : 0x06020400u);
+    const unsigned far = static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w), 0x4e, 0xf, 0xf, true));  // lane ^ 2
+    return __builtin_amdgcn_perm(far, w, lane & 2 ? 0x03020706u : 0x05040100u);
+}
+
+// Word j of the lane in group g of 16 becomes word g of the lane in group j.
+__device__ __forceinline__ uint4 transpose_groups(uint4 w) {
+    const auto a = __builtin_amdgcn_permlane32_swap(w.x, w.z, false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(w.y, w.w, false, false);
+    const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    return uint4{c[0], c[1], d[0], d[1]};
+}
+
+typedef unsigned short ushortx2_t __attribute__((ext_vector_type(2)));
+
 template <int kFormat, int kGranules>  // granules of a page
-__device__ void append_run(const Kv8Cache& cache, const Kv8AppendArgs& a, int row, int count, int slot, int head,
-                           bool is_value, unsigned char* lds) {
+__device__ __forceinline__ void append_run(const Kv8Cache& cache, const Kv8AppendArgs& a, int row, int count, int slot, int head,
+                                           bool is_value, unsigned* lds) {
     constexpr int kPage = kGranules * kKv8Granule;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, granule = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int page = slot / kPage, offset = slot % kPage, end = offset + count;
-    const int first_granule = offset / kKv8Granule, granules_end = (end + kKv8Granule - 1) / kKv8Granule;
+    const int first = granule * kKv8Granule;  // the wave's granule's first token
     const size_t of_page = static_cast<size_t>(page) * cache.key_value_heads + head;
     unsigned char* bytes = (is_value ? cache.value_pages : cache.key_pages) + of_page * (kGranules * kKv8GranuleBytes);
     float* scale_at = (is_value ? cache.value_scales : cache.key_scales) + of_page;
     const int stride = is_value ? a.value_stride : a.key_stride;
     const bf16_t* rows = (is_value ? a.value : a.key) + static_cast<size_t>(head) * kKv8HeadDimension;
 
-    // the page's scale and the granule that the run enters half-way, beside the rows
-    const bool keeps = offset > 0, enters = offset % kKv8Granule != 0;
+    // lane (token of the granule, group of 16 dimensions), and where its 16
+    // bytes lie: keys token by token, values as (token / 4, d % 16) after the
+    // transpositions, which bring lane (group, token / 4, token % 4) the words of
+    // d % 16 = 4 group + token % 4
+    const int token = lane & 15, group = lane >> 4;
+    const int place = is_value ? (token >> 2) * 256 + (4 * group + (token & 3)) * 16 : token * 64 + group * 16;
+    uint4* to = reinterpret_cast<uint4*>(bytes + granule * kKv8GranuleBytes + place);  // and 64 further for the upper dimensions
+
+    // the rows, beside the page's scale and a granule that the run enters half-way
+    const bool keeps = offset > 0;
+    const bool touched = first < end && first + kKv8Granule > offset;  // by the run
+    const bool merges = touched && first < offset;
+    const bool mine = first + token >= offset && first + token < end;
     const float old_scale = keeps ? *scale_at : 0.0f;
-    uint4 before[2];
-    if (enters) {
-        const uint4* from = reinterpret_cast<const uint4*>(bytes + first_granule * kKv8GranuleBytes) + lane;
-        before[0] = from[0], before[1] = from[64];
-    }
-    // lane (token of the granule, group of 16 dimensions)
-    const int token = lane >> 2, group = lane & 3;
-    uint4 x[kGranules][2][2];
-    int largest_bits = 0;
+    uint4 x[2][2], before[2];
 #pragma unroll
-    for (int g = 0; g < kGranules; ++g) {
-        const int t = g * kKv8Granule + token;
-        const bool mine = t >= offset && t < end;
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                x[g][c][u] = uint4{0, 0, 0, 0};
-                if (mine) {
-                    x[g][c][u] = *reinterpret_cast<const uint4*>(rows + static_cast<size_t>(row + t - offset) * stride +
-                                                                 c * 64 + group * 16 + u * 8);
-                }
+        for (int u = 0; u < 2; ++u) {
+            x[c][u] = uint4{0, 0, 0, 0};
+            if (mine) {
+                x[c][u] = *reinterpret_cast<const uint4*>(rows + static_cast<size_t>(row + first + token - offset) * stride +
+                                                          c * 64 + group * 16 + u * 8);
             }
-    }
+        }
+    if (merges) before[0] = to[0], before[1] = to[64];
+
+    ushortx2_t most{0, 0};
 #pragma unroll
-    for (int g = 0; g < kGranules; ++g)
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const unsigned w[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(ushortx2_t, w[i] & 0x7fff7fffu));
+        }
+    unsigned largest = block_max<kGranules>(max(most[0], most[1]), lds);
+    const bool odd = largest >= 0x7f80u;  // an infinity or a NaN is among them: looked for one by one
+    if (odd) {
+        unsigned finite = 0;
         for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const unsigned w[4] = {x[g][c][u].x, x[g][c][u].y, x[g][c][u].z, x[g][c][u].w};
-#pragma unroll
+            for (int u = 0; u < 2; ++u)
                 for (int i = 0; i < 4; ++i) {
-                    const int lo = w[i] & 0x7fff, hi = (w[i] >> 16) & 0x7fff;
-                    largest_bits = max(largest_bits, lo < 0x7f80 ? lo : 0);
-                    largest_bits = max(largest_bits, hi < 0x7f80 ? hi : 0);
+                    const unsigned w = i == 0 ? x[c][u].x : i == 1 ? x[c][u].y : i == 2 ? x[c][u].z : x[c][u].w;
+                    const unsigned lo = w & 0x7fffu, hi = w >> 16 & 0x7fffu;
+                    finite = max(finite, lo < 0x7f80u ? lo : 0u);
+                    finite = max(finite, hi < 0x7f80u ? hi : 0u);
                 }
-            }
-    largest_bits = wave_max(largest_bits);
-    const float wanted = scale_for<kFormat>(__uint_as_float(static_cast<unsigned>(largest_bits) << 16));
+        largest = block_max<kGranules>(finite, lds);
+    }
+    const float wanted = scale_for<kFormat>(__uint_as_float(largest << 16));
     // a scale that is no number cannot be kept: its tokens are lost, the new ones are not
     const float scale = wanted >= old_scale ? wanted : old_scale == old_scale ? old_scale : wanted;
     const double inverse = scale > 0.0f ? 1.0 / static_cast<double>(scale) : 0.0;
     const bool grew = keeps && scale != old_scale;
-    const double ratio = scale > 0.0f ? static_cast<double>(old_scale) / static_cast<double>(scale) : 1.0;
+    double ratio = scale > 0.0f ? static_cast<double>(old_scale) / static_cast<double>(scale) : 1.0;
+    if (!(ratio <= 1.0)) ratio = 0.0;
 
-    // bytes of tokens before the run in the new scale
-    auto moved = [&](uint4 w) {
-        return uint4{rescale4<kFormat>(w.x, ratio), rescale4<kFormat>(w.y, ratio), rescale4<kFormat>(w.z, ratio),
-                     rescale4<kFormat>(w.w, ratio)};
-    };
-    if (grew) {
-        for (int g = 0; g < first_granule; ++g) {
-            uint4* at = reinterpret_cast<uint4*>(bytes + g * kKv8GranuleBytes) + lane;
-            const uint4 w0 = at[0], w1 = at[64];
-            at[0] = moved(w0), at[64] = moved(w1);
-        }
-    }
-#pragma unroll
-    for (int g = 0; g < kGranules; ++g) {
-        if (g < first_granule || g >= granules_end) continue;
+    if (touched) {
         uint4 fresh[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             unsigned w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint4& half = x[g][c][i >> 1];
-                const unsigned lo = i & 1 ? half.z : half.x, hi = i & 1 ? half.w : half.y;
-                const auto at = [&](unsigned bits) {
-                    const float v = __uint_as_float(bits);
-                    return v == v ? static_cast<double>(v) * inverse : 0.0;
-                };
-                // an infinity times a zero reciprocal (a run without a finite magnitude) is held as 0
-                const auto fine = [](double v) { return v == v ? v : 0.0; };
-                w[i] = hold4<kFormat>(fine(at(lo << 16)), fine(at(lo & 0xffff0000u)), fine(at(hi << 16)),
-                                      fine(at(hi & 0xffff0000u)));
+                const uint4& eight = x[c][i >> 1];
+                const unsigned lo = i & 1 ? eight.z : eight.x, hi = i & 1 ? eight.w : eight.y;
+                const auto quotient = [&](unsigned bits) { return static_cast<double>(__uint_as_float(bits)) * inverse; };
+                double v[4] = {quotient(lo << 16), quotient(lo & 0xffff0000u), quotient(hi << 16), quotient(hi & 0xffff0000u)};
+                if (odd) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        // NaN, also of an infinity in a run without a finite magnitude, becomes 0
+                        constexpr double kRange = kFormat == kKv8Int8 ? 127.0 : 448.0;
+                        v[e] = v[e] == v[e] ? fmin(fmax(v[e], -kRange), kRange) : 0.0;
+                    }
+                }
+                w[i] = hold4<kFormat>(v[0], v[1], v[2], v[3]);
             }
             fresh[c] = uint4{w[0], w[1], w[2], w[3]};
         }
-        const int base = g * kKv8Granule;
-        const bool merge = enters && g == first_granule;
-        uint4 keep[2] = {uint4{0, 0, 0, 0}, uint4{0, 0, 0, 0}};
-        if (merge) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) keep[c] = before[c];
-        }
-        uint4* to = reinterpret_cast<uint4*>(bytes + g * kKv8GranuleBytes) + lane;
         if (!is_value) {
-            const int t = base + token;
+            if (merges) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                if (merge) {
-                    if (t < offset) fresh[c] = grew ? moved(keep[c]) : keep[c];
-                    else if (t >= end) fresh[c] = keep[c];
+                for (int c = 0; c < 2; ++c) {
+                    if (first + token < offset) fresh[c] = grew ? rescale16<kFormat>(before[c], ratio) : before[c];
+                    else if (first + token >= end) fresh[c] = before[c];
                 }
-                to[c * 64] = fresh[c];
             }
         } else {
-            // token `token`, dimensions 64 c + 16 group + e: byte (token / 4) * 256 + e * 16 + group * 4 + token % 4
-            __syncthreads();
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const unsigned w[4] = {fresh[c].x, fresh[c].y, fresh[c].z, fresh[c].w};
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    lds[c * 1024 + (token >> 2) * 256 + e * 16 + group * 4 + (token & 3)] =
-                        static_cast<unsigned char>(w[e >> 2] >> (8 * (e & 3)));
-                }
+                fresh[c] = transpose_groups(uint4{transpose_bytes(fresh[c].x, lane), transpose_bytes(fresh[c].y, lane),
+                                                  transpose_bytes(fresh[c].z, lane), transpose_bytes(fresh[c].w, lane)});
             }
-            __syncthreads();
-            // lane (token / 4, d % 16)
-            const int t = base + 4 * (lane >> 4);
-            const unsigned earlier = byte_mask(t, 0, offset), later = byte_mask(t, end, INT_MAX);
+            if (merges) {
+                const int four = first + (token & ~3);
+                const unsigned earlier = byte_mask(four, 0, offset), later = byte_mask(four, end, INT_MAX);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint4 w = reinterpret_cast<const uint4*>(lds)[c * 64 + lane];
-                if (merge) {
-                    const uint4 scaled = grew ? moved(keep[c]) : keep[c];
+                for (int c = 0; c < 2; ++c) {
+                    const uint4 scaled = grew ? rescale16<kFormat>(before[c], ratio) : before[c];
                     const auto pick = [&](unsigned n, unsigned m, unsigned o) {
                         return (n & ~(earlier | later)) | (m & earlier) | (o & later);
                     };
-                    w = uint4{pick(w.x, scaled.x, keep[c].x), pick(w.y, scaled.y, keep[c].y),
-                              pick(w.z, scaled.z, keep[c].z), pick(w.w, scaled.w, keep[c].w)};
+                    fresh[c] = uint4{pick(fresh[c].x, scaled.x, before[c].x), pick(fresh[c].y, scaled.y, before[c].y),
+                                     pick(fresh[c].z, scaled.z, before[c].z), pick(fresh[c].w, scaled.w, before[c].w)};
                 }
-                to[c * 64] = w;
             }
         }
+        to[0] = fresh[0], to[64] = fresh[1];
+    } else if (grew && first < offset) {
+        const uint4 w0 = to[0], w1 = to[64];
+        to[0] = rescale16<kFormat>(w0, ratio), to[64] = rescale16<kFormat>(w1, ratio);
     }
-    if (lane == 0 && (!keeps || grew)) *scale_at = scale;
+    if (threadIdx.x == 0 && (!keeps || grew)) *scale_at = scale;
 }
 
-// A wave looks at kRows rows and takes the runs that begin there.
-template <int kFormat, int kGranules, int kRows>
-__global__ __launch_bounds__(64) void kv8_append_kernel(Kv8Cache cache, Kv8AppendArgs a) {
-    __shared__ __align__(16) unsigned char lds[kKv8GranuleBytes];
+// `slices` workgroups look at the same kRows rows and take the runs that begin
+// there in turn.
+template <int kFormat, int kGranules>
+__global__ __launch_bounds__(64 * kGranules) void kv8_append_kernel(Kv8Cache cache, Kv8AppendArgs a, int slices) {
+    __shared__ unsigned lds[kGranules];
     constexpr int kPage = kGranules * kKv8Granule;
-    const int lane = threadIdx.x;
-    const int first = blockIdx.x * kRows;
+    const int lane = threadIdx.x & 63;
+    const int first = static_cast<int>(blockIdx.x / slices) * kRows, slice = blockIdx.x % slices;
     const int head = blockIdx.y;
     const bool is_value = blockIdx.z != 0;
     const int slots = cache.pages * kPage;
@@ -242,35 +277,40 @@ __global__ __launch_bounds__(64) void kv8_append_kernel(Kv8Cache cache, Kv8Appen
         const int s = a.row_slots[row];
         return s >= 0 && s < slots ? s : -1;
     };
-    bool begins = false;
-    if (lane < kRows) {
-        const int mine = slot_of(first + lane), last = slot_of(first + lane - 1);
-        begins = mine >= 0 && !(last >= 0 && mine == last + 1 && mine % kPage != 0);
-    }
-    for (unsigned long long todo = __ballot(begins); todo != 0; todo &= todo - 1) {
-        const int row = first + __ffsll(todo) - 1;
-        const int slot = a.row_slots[row];
+    // the rows, the one before them, and those behind them that a run which begins here can have
+    const int before = slot_of(first - 1), mine = slot_of(first + lane), later = slot_of(first + kRows + lane);
+    int last = __builtin_amdgcn_update_dpp(0, mine, 0x138, 0xf, 0xf, false);  // wave_shr:1
+    if (lane == 0) last = before;
+    const bool begins = mine >= 0 && !(last >= 0 && mine == last + 1 && mine % kPage != 0);
+    // this workgroup's turns among the runs
+    const unsigned turn = __popcll(__ballot(begins) & ((1ull << lane) - 1));
+    for (unsigned long long todo = __ballot(begins && turn % static_cast<unsigned>(slices) == static_cast<unsigned>(slice)); todo != 0; todo &= todo - 1) {
+        const int from = __ffsll(todo) - 1;
+        const int slot = __builtin_amdgcn_readlane(mine, from);
         // the run: rows that follow one another up to the page's end
-        const bool follows = lane < kPage - slot % kPage && slot_of(row + lane) == slot + lane;
-        const unsigned long long stops = ~__ballot(follows);
-        const int count = stops == 0 ? 64 : __ffsll(stops) - 1;
-        append_run<kFormat, kGranules>(cache, a, row, count, slot, head, is_value, lds);
+        const int most = kPage - slot % kPage;
+        const unsigned long long here = __ballot(lane >= from && lane - from < most && mine == slot + lane - from) >> from;
+        const unsigned long long there = __ballot(kRows + lane - from < most && later == slot + kRows + lane - from);
+        int count = ~here == 0 ? kRows : __ffsll(~here) - 1;
+        if (count == kRows - from) count += ~there == 0 ? kRows : __ffsll(~there) - 1;
+        append_run<kFormat, kGranules>(cache, a, first + from, count, slot, head, is_value, lds);
     }
 }
 
 template <int kFormat, int kGranules>
 hipError_t launch_pages(const Kv8Cache& cache, const Kv8AppendArgs& a, hipStream_t stream) {
-    // One row a wave while that leaves the launch small: a row's wave starts
-    // at once and single tokens of many sequences do not queue behind one
-    // another.  Prompts: 15 of 16 rows begin no run.
-    constexpr int kRows = 16;
-    if (static_cast<long long>(a.rows) * cache.key_value_heads <= 4096) {
-        kv8_append_kernel<kFormat, kGranules, 1>
-            <<<dim3(a.rows, cache.key_value_heads, 2), 64, 0, stream>>>(cache, a);
-    } else {
-        kv8_append_kernel<kFormat, kGranules, kRows>
-            <<<dim3((a.rows + kRows - 1) / kRows, cache.key_value_heads, 2), 64, 0, stream>>>(cache, a);
-    }
+    // Single tokens of many sequences begin a run in every row, prompts in one
+    // of a page's: several workgroups share 64 rows' runs, as many as a prompt
+    // has there at least, and more while the launch stays small, since one that
+    // finds none costs its start.  1024 / 2048 / 4096 workgroups, us: 256 single
+    // tokens 9.2 / 7.4 / 6.9, four prompts of 512 rows 5.1 / 5.0 / 7.7, with pages
+    // of 64 tokens (four waves) 7.4 / 11.7 / 18.4.
+    constexpr int kLeast = kRows / (kGranules * kKv8Granule);
+    constexpr int kWorkgroups = kGranules == 4 ? 1024 : 2048;
+    const long long groups = (a.rows + kRows - 1) / kRows, units = groups * cache.key_value_heads * 2;
+    const int slices = static_cast<int>(std::clamp<long long>(kWorkgroups / units, kLeast, kRows));
+    kv8_append_kernel<kFormat, kGranules>
+        <<<dim3(static_cast<unsigned>(groups * slices), cache.key_value_heads, 2), 64 * kGranules, 0, stream>>>(cache, a, slices);
     return hipGetLastError();
 }
 

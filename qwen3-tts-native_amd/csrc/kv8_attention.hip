@@ -25,13 +25,20 @@ constexpr int kDim = kKv8HeadDimension;
 constexpr int kMaxGroup = 16;  // query heads of a key/value head: the columns of the smallest product
 constexpr float kLog2E = 1.44269504088896340736f;
 
+constexpr int kFewWaves = 4;
+// Workgroups for sequences of many rows: column waves x key groups of 4 x 1, 4 x 2, 2 x 4.
+enum Many : int { kNone = 0, kWide, kHalved, kQuartered };
+
 struct Params {
     Kv8AttentionArgs a;
     Kv8Cache cache;
     int group = 1;     // query heads of a key/value head
-    float scale2 = 0;  // scale * log2(e)
+    float scale2 = 0;  // |scale| * log2(e)
+    unsigned flip = 0;  // sign bits of a pair of bf16: the query's are flipped for a negative scale
     int splits = 1;    // workgroups that share a context of few rows
     int columns = 16;  // (row, head of the group) pairs that a shared context can have
+    int waves = kFewWaves;  // of a workgroup of few rows
+    int many = kNone;
     int few = INT_MAX;  // pairs up to which a sequence counts as one of few rows
     float* partial_out = nullptr;   // [sequence][kv head][column][split][128]
     float2* partial_sums = nullptr;  // [sequence][kv head][column][split] (maximum, sum)
@@ -65,15 +72,37 @@ __device__ __forceinline__ size_t partial_slot(const Params& p, int sequence, in
     return ((static_cast<size_t>(sequence) * p.cache.key_value_heads + kv_head) * p.columns + column) * p.splits;
 }
 
+// Pages and scales of a wave's next 64 granules, one a lane, so that no step
+// waits for its table entry, then for its scales, before it can ask for bytes.
+struct Lookup {
+    int page;  // -1: none
+    float key_scale, value_scale;
+};
+// `token` is the first of the lane's granule, `end` the end of what counts.
+template <int kPage>
+__device__ __forceinline__ Lookup look_up(const Params& p, const int* table, int kv_head, int token, int end) {
+    const int at = min(token, (end - 1) & ~(kKv8Granule - 1));  // past the end: the last one again
+    int page = table[at / kPage];
+    if (page < 0 || page >= p.cache.pages) page = -1;
+    const size_t scale_at = static_cast<size_t>(max(page, 0)) * p.cache.key_value_heads + kv_head;
+    const bool counts = page >= 0 && token < end;
+    return Lookup{page, counts ? p.cache.key_scales[scale_at] * p.scale2 : 0.0f, counts ? p.cache.value_scales[scale_at] : 0.0f};
+}
+__device__ __forceinline__ int of_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float of_lane(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
 // ---------------------------------------------------------------------------
 // Few rows: up to 16 (row, head) pairs of one key/value head are the columns
 // of 16x16x32 products, keys and values are read once for all of them.
 // ---------------------------------------------------------------------------
-constexpr int kWaves = 4;
 constexpr int kStep = 64;  // tokens of a wave's step
 constexpr int kStepGranules = kStep / kKv8Granule;
 
-template <int kFormat, int kPageGranules>
+template <int kFormat, int kPageGranules, int kWaves>
+// Two waves a SIMD: with registers for three (168) the compiler spills, and
+// 256 sequences up to 8192 tokens take 601 us instead of 445.
 __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) {
     __shared__ __align__(16) float out_lds[kWaves][8 * 64 * 4];
     __shared__ float max_lds[kWaves][16], sum_lds[kWaves][16];
@@ -108,6 +137,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
                     w = *reinterpret_cast<const uint4*>(p.a.query +
                                                         static_cast<size_t>(rows.first + row) * p.a.query_stride +
                                                         head * kDim + c * 64 + quad * 16 + u * 8);
+                    w = uint4{w.x ^ p.flip, w.y ^ p.flip, w.z ^ p.flip, w.w ^ p.flip};
                 }
                 q[c][u] = __builtin_bit_cast(bf16x8_t, w);
             }
@@ -124,28 +154,47 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
         floatx4_t acc[8];
 #pragma unroll
         for (int d = 0; d < 8; ++d) acc[d] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-        for (int step = steps_begin + wave; step < steps_end; step += kWaves) {
-            const int token0 = begin + step * kStep;
-            uint4 k[kStepGranules][2], v[kStepGranules][2];
+        // the wave's i-th step and its granules; their bytes are asked for as
+        // soon as the registers of the step before are free
+        const int mine_steps = steps_end > steps_begin + wave ? (steps_end - steps_begin - wave + kWaves - 1) / kWaves : 0;
+        constexpr int kLooked = 64 / kStepGranules;  // steps of a look-up
+        const auto token_of = [&](int i) { return begin + (steps_begin + wave + i * kWaves) * kStep; };
+        uint4 k[kStepGranules][2], v[kStepGranules][2];
+        Lookup looked{};
+        const auto look = [&](int i) {
+            looked = look_up<kPage>(p, table, kv_head, token_of(i + lane / kStepGranules) + lane % kStepGranules * kKv8Granule, end);
+        };
+        const auto offset_of = [&](int i, int g) {
+            const int page = max(of_lane(looked.page, i % kLooked * kStepGranules + g), 0);
+            const int at = min(token_of(i) + g * kKv8Granule, (end - 1) & ~(kKv8Granule - 1));
+            return page * page_bytes + at % kPage / kKv8Granule * kKv8GranuleBytes;
+        };
+        const auto load = [&](uint4 (&to)[kStepGranules][2], const unsigned char* from, int i) {
+#pragma unroll
+            for (int g = 0; g < kStepGranules; ++g) {
+                const unsigned char* at = from + offset_of(i, g);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) to[g][c] = *reinterpret_cast<const uint4*>(at + c * 1024);
+            }
+        };
+        if (mine_steps > 0) {
+            look(0);
+            load(k, keys_of_lane, 0);
+            load(v, values, 0);
+        }
+        for (int i = 0; i < mine_steps; ++i) {
+            const int token0 = token_of(i);
             float key_scale[kStepGranules], value_scale[kStepGranules];
             int held[kStepGranules];  // tokens of the granule that hold something
 #pragma unroll
             for (int g = 0; g < kStepGranules; ++g) {
-                const int first = token0 + g * kKv8Granule;
-                const int at = min(first, (end - 1) & ~(kKv8Granule - 1));  // past the end: the last one again
-                int page = table[at / kPage];
-                held[g] = min(max(end - first, 0), kKv8Granule);
-                if (page < 0 || page >= p.cache.pages) page = 0, held[g] = 0;
-                const size_t offset = page * page_bytes + at % kPage / kKv8Granule * kKv8GranuleBytes;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    k[g][c] = *reinterpret_cast<const uint4*>(keys_of_lane + offset + c * 1024);
-                    v[g][c] = *reinterpret_cast<const uint4*>(values + offset + c * 1024);
-                }
-                const size_t scale_at = static_cast<size_t>(page) * p.cache.key_value_heads + kv_head;
-                key_scale[g] = p.cache.key_scales[scale_at] * p.scale2;
-                value_scale[g] = held[g] > 0 ? p.cache.value_scales[scale_at] : 0.0f;
+                const int from = i % kLooked * kStepGranules + g;
+                key_scale[g] = of_lane(looked.key_scale, from);
+                value_scale[g] = of_lane(looked.value_scale, from);
+                held[g] = of_lane(looked.page, from) < 0 ? 0 : min(max(end - token0 - g * kKv8Granule, 0), kKv8Granule);
             }
+            const bool more = i + 1 < mine_steps;
+            if (more && (i + 1) % kLooked == 0) look(i + 1);
             float s[kStepGranules][4];
             float top = maximum;
 #pragma unroll
@@ -158,13 +207,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
                 }
                 const int first = token0 + g * kKv8Granule + 4 * quad;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int token = first + i;
-                    const bool counts = token <= position && token > lowest && 4 * quad + i < held[g];
-                    s[g][i] = counts ? dot[i] * key_scale[g] : -INFINITY;
-                    top = fmaxf(top, s[g][i]);
+                for (int e = 0; e < 4; ++e) {
+                    const int token = first + e;
+                    const bool counts = token <= position && token > lowest && 4 * quad + e < held[g];
+                    s[g][e] = counts ? dot[e] * key_scale[g] : -INFINITY;
+                    top = fmaxf(top, s[g][e]);
                 }
             }
+            if (more) load(k, keys_of_lane, i + 1);
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             const float reference = top == -INFINITY ? 0.0f : top;  // nothing counted yet: weights become 0
@@ -179,16 +229,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
             for (int g = 0; g < kStepGranules; ++g) {
                 float w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(s[g][i] - reference);
-                    sum += e;
-                    w[i] = e * value_scale[g];
+                for (int e = 0; e < 4; ++e) {
+                    const float weight = __builtin_amdgcn_exp2f(s[g][e] - reference);
+                    sum += weight;
+                    w[e] = weight * value_scale[g];
                 }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    high[g][i] = pack_bf16(w[2 * i], w[2 * i + 1]);
-                    low[g][i] = pack_bf16(w[2 * i] - __uint_as_float(high[g][i] << 16),
-                                          w[2 * i + 1] - __uint_as_float(high[g][i] & 0xffff0000u));
+                for (int e = 0; e < 2; ++e) {
+                    high[g][e] = pack_bf16(w[2 * e], w[2 * e + 1]);
+                    low[g][e] = pack_bf16(w[2 * e] - __uint_as_float(high[g][e] << 16),
+                                          w[2 * e + 1] - __uint_as_float(high[g][e] & 0xffff0000u));
                 }
                 if (held[g] < kKv8Granule) {
                     // bytes behind the length may hold anything, an e4m3 NaN too, which a zero weight would not silence
@@ -213,6 +263,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
                     }
                 }
             }
+            if (more) load(v, values, i + 1);
         }
         // over the lanes of a column, then over the waves
         sum += __shfl_xor(sum, 16, 64);
@@ -230,12 +281,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
 #pragma unroll
         for (int d = 0; d < 8; ++d) *reinterpret_cast<floatx4_t*>(&out_lds[wave][(d * 64 + lane) * 4]) = acc[d] * mine_shrinks;
         __syncthreads();
-        // wave w: dimensions 32 w .. 32 w + 31 (two tiles of 16) of every column
+        // wave w: dimension tiles of 16, every column
         if (mine) {
             const size_t slot = partial_slot(p, sequence, kv_head, column) + split;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int d = 2 * wave + j;
+            for (int j = 0; j < 8 / kWaves; ++j) {
+                const int d = 8 / kWaves * wave + j;
                 floatx4_t o = *reinterpret_cast<const floatx4_t*>(&out_lds[0][(d * 64 + lane) * 4]);
 #pragma unroll
                 for (int w = 1; w < kWaves; ++w) o += *reinterpret_cast<const floatx4_t*>(&out_lds[w][(d * 64 + lane) * 4]);
@@ -253,58 +304,103 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
     }
 }
 
-// Joins the results of workgroups that shared a context: a wave a (row, head).
-__global__ __launch_bounds__(64 * kWaves) void kv8_join_kernel(Params p) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kv_head = blockIdx.x, sequence = blockIdx.y;
+// Joins the results of workgroups that shared a context: a workgroup a (row,
+// head), its 8 groups of 32 lanes take every eighth of the partial results
+// (one wave for all of them: 18 us for 64 of a row, now 4).
+constexpr int kJoinGroups = 8;
+__global__ __launch_bounds__(32 * kJoinGroups) void kv8_join_kernel(Params p) {
+    __shared__ float max_lds[kJoinGroups], sum_lds[kJoinGroups];
+    __shared__ __align__(16) float out_lds[kJoinGroups][kDim];
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+    const int column = blockIdx.x, kv_head = blockIdx.y, sequence = blockIdx.z;
     const Rows rows = rows_of(p, sequence);
     const int splits = splits_of(p, rows);
-    if (splits <= 1) return;
-    for (int column = wave; column < rows.count * p.group; column += kWaves) {
-        const size_t slot = partial_slot(p, sequence, kv_head, column);
-        float top = -INFINITY;
-        for (int i = lane; i < splits; i += 64) top = fmaxf(top, p.partial_sums[slot + i].x);
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-        const float reference = top == -INFINITY ? 0.0f : top;
-        float total = 0.0f;
-        floatx2_t o{0.f, 0.f};
-        for (int i = 0; i < splits; ++i) {
-            const float2 part = p.partial_sums[slot + i];
-            const float share = __builtin_amdgcn_exp2f(part.x - reference);
-            total += part.y * share;
-            o += *reinterpret_cast<const floatx2_t*>(p.partial_out + (slot + i) * kDim + 2 * lane) * share;
-        }
-        const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
-        const int row = rows.first + column / p.group, head = kv_head * p.group + column % p.group;
-        *reinterpret_cast<unsigned*>(p.a.out + static_cast<size_t>(row) * p.a.out_stride + head * kDim + 2 * lane) =
-            pack_bf16(o[0] * inverse, o[1] * inverse);
+    if (splits <= 1 || column >= rows.count * p.group) return;
+    const size_t slot = partial_slot(p, sequence, kv_head, column);
+    float top = -INFINITY, total = 0.0f;
+    floatx4_t o{0.f, 0.f, 0.f, 0.f};
+    for (int i = group; i < splits; i += kJoinGroups) {
+        const float2 part = p.partial_sums[slot + i];
+        const floatx4_t values = *reinterpret_cast<const floatx4_t*>(p.partial_out + (slot + i) * kDim + 4 * lane);
+        const float next = fmaxf(top, part.x), reference = next == -INFINITY ? 0.0f : next;
+        const float shrink = __builtin_amdgcn_exp2f(top - reference), share = __builtin_amdgcn_exp2f(part.x - reference);
+        total = total * shrink + part.y * share;
+        o = o * shrink + values * share;
+        top = next;
     }
+    if (lane == 0) max_lds[group] = top, sum_lds[group] = total;
+    *reinterpret_cast<floatx4_t*>(&out_lds[group][4 * lane]) = o;
+    __syncthreads();
+    if (threadIdx.x >= kDim / 2) return;
+    top = max_lds[0];
+#pragma unroll
+    for (int g = 1; g < kJoinGroups; ++g) top = fmaxf(top, max_lds[g]);
+    const float reference = top == -INFINITY ? 0.0f : top;
+    floatx2_t sums{0.f, 0.f};
+    total = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kJoinGroups; ++g) {
+        const float share = __builtin_amdgcn_exp2f(max_lds[g] - reference);
+        total += sum_lds[g] * share;
+        sums += *reinterpret_cast<const floatx2_t*>(&out_lds[g][2 * threadIdx.x]) * share;
+    }
+    const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
+    const int row = rows.first + column / p.group, head = kv_head * p.group + column % p.group;
+    *reinterpret_cast<unsigned*>(p.a.out + static_cast<size_t>(row) * p.a.out_stride + head * kDim + 2 * threadIdx.x) =
+        pack_bf16(sums[0] * inverse, sums[1] * inverse);
 }
 
 // ---------------------------------------------------------------------------
 // Many rows: a wave owns 32 (row, head) pairs of a key/value head as the
-// columns of 32x32x16 products, the block's waves share its keys and values,
+// columns of 32x32x16 products; the block's waves share its keys and values,
 // which go through LDS as bf16: a byte is converted once for all columns.
 // Scores are formed transposed, S^T = K Q^T, with key rows dealt so that a
 // lane's scores are those of eight consecutive tokens, the operand of the value
 // product O^T = V^T P^T: weights never leave their lane.
+// Waves are kColumnWaves x kKeyWaves: those of a key group take the same 64 of
+// every 64 * kKeyWaves tokens, and the groups' results are joined at the end.
 // ---------------------------------------------------------------------------
-constexpr int kTile = 64;  // tokens in LDS at a time
+constexpr int kTile = 64;  // tokens of a wave's step
 constexpr int kTileGranules = kTile / kKv8Granule;
+constexpr int kTileBytes = kTile * kDim * 2;  // as bf16
 // a maximum may stay this far (log2) behind the scores before the sums are scaled anew
 constexpr float kSlack = 8.0f;
+// Smallest value scale that goes into the weights as it is, see stage().
+constexpr float kLeastScale = 0x1p-60f;
 
-template <int kFormat, int kPageGranules, int kManyWaves>
-__global__ __launch_bounds__(64 * kManyWaves, 2) void kv8_many_rows_kernel(Params p) {
-    static_assert(kManyWaves == kTileGranules, "a wave stages a granule");
-    __shared__ __align__(16) unsigned char key_lds[2][kTile * kDim * 2];    // [token][16-byte groups of dimensions, swizzled]
-    __shared__ __align__(16) unsigned char value_lds[2][kTile * kDim * 2];  // [dimension][16-byte groups of tokens, swizzled]
-    __shared__ float key_scale_lds[2][kTileGranules], value_scale_lds[2][kTileGranules];
-    __shared__ int held_lds[2][kTileGranules];
+// Four held values times `factor` as bf16.
+template <int kFormat>
+__device__ __forceinline__ uint2 scaled_bf16_of(unsigned w, float factor) {
+    const uint2 v = bf16_of<kFormat>(w);
+    return uint2{pack_bf16(__uint_as_float(v.x << 16) * factor, __uint_as_float(v.x & 0xffff0000u) * factor),
+                 pack_bf16(__uint_as_float(v.y << 16) * factor, __uint_as_float(v.y & 0xffff0000u) * factor)};
+}
+
+template <int kColumnWaves, int kKeyWaves>
+struct ManyShared {
+    static constexpr int kBuffers = kKeyWaves == 1 ? 2 : 1;
+    unsigned char keys[kBuffers][kKeyWaves][kTileBytes];    // [token][16-byte groups of dimensions, swizzled]
+    unsigned char values[kBuffers][kKeyWaves][kTileBytes];  // [dimension][16-byte groups of tokens, swizzled]
+    float key_scale[kBuffers][kKeyWaves][kTileGranules];
+    float value_log[kBuffers][kKeyWaves][kTileGranules];      // log2 of the values' scale
+    float value_inverse[kBuffers][kKeyWaves][kTileGranules];  // and its reciprocal
+    int held[kBuffers][kKeyWaves][kTileGranules];
+    float maximum[kKeyWaves][kColumnWaves][32], sum[kKeyWaves][kColumnWaves][32];
+};
+
+template <int kFormat, int kPageGranules, int kColumnWaves, int kKeyWaves>
+__global__ __launch_bounds__(64 * kColumnWaves * kKeyWaves, 2) void kv8_many_rows_kernel(Params p) {
+    using Shared = ManyShared<kColumnWaves, kKeyWaves>;
+    extern __shared__ __align__(16) unsigned char dynamic_lds[];
+    Shared& lds = *reinterpret_cast<Shared*>(dynamic_lds);
+    constexpr int kBuffers = Shared::kBuffers;
     constexpr int kPage = kPageGranules * kKv8Granule;
-    constexpr int kColumns = 32 * kManyWaves;
+    constexpr int kColumns = 32 * kColumnWaves;
+    constexpr int kStepTokens = kTile * kKeyWaves;
+    constexpr int kStaged = kTileGranules / kColumnWaves;  // granules that a wave stages
+    static_assert(kStaged * kColumnWaves == kTileGranules, "column waves stage a tile's granules");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int column_wave = wave % kColumnWaves, key_wave = wave / kColumnWaves;
     const int column = lane & 31, half = lane >> 5;
     const int kv_head = blockIdx.x, sequence = blockIdx.z;
     const Rows rows = rows_of(p, sequence);
@@ -318,7 +414,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void kv8_many_rows_kernel(Param
 
     // the longest rows first: they are the launch's tail
     for (int tile = tiles - 1 - static_cast<int>(blockIdx.y); tile >= 0; tile -= gridDim.y) {
-        const int pair = tile * kColumns + wave * 32 + column;
+        const int pair = tile * kColumns + column_wave * 32 + column;
         const bool mine = pair < pairs;
         const int row = min(pair, pairs - 1) / p.group;
         const int head = kv_head * p.group + pair % p.group;
@@ -331,6 +427,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void kv8_many_rows_kernel(Param
             if (mine) {
                 w = *reinterpret_cast<const uint4*>(p.a.query + static_cast<size_t>(rows.first + row) * p.a.query_stride +
                                                     head * kDim + 16 * k + 8 * half);
+                w = uint4{w.x ^ p.flip, w.y ^ p.flip, w.z ^ p.flip, w.w ^ p.flip};
             }
             q[k] = __builtin_bit_cast(bf16x8_t, w);
         }
@@ -339,59 +436,79 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void kv8_many_rows_kernel(Param
         const int last_row = min(tile * kColumns + kColumns - 1, pairs - 1) / p.group;
         const int end = min(rows.position + last_row + 1, rows.length);
         const int begin = p.a.window > 0 ? max(rows.position + first_row - p.a.window + 1, 0) & ~(kTile - 1) : 0;
-        const int steps = end > begin ? (end - begin + kTile - 1) / kTile : 0;
-        const int wave_pair = tile * kColumns + wave * 32;
+        const int steps = end > begin ? (end - begin + kStepTokens - 1) / kStepTokens : 0;
+        const int wave_pair = tile * kColumns + column_wave * 32;
         const bool wave_lives = wave_pair < pairs;
         const int wave_first = rows.position + min(wave_pair, pairs - 1) / p.group;
         const int wave_last = rows.position + min(wave_pair + 31, pairs - 1) / p.group;
 
-        uint4 k_bytes[2], v_bytes[2];
-        float key_scale = 0.f, value_scale = 0.f;
-        int held = 0;
+        uint4 k_bytes[kStaged][2], v_bytes[kStaged][2];
+        float key_scale[kStaged], value_scale[kStaged];
+        int held[kStaged];
+        constexpr int kLooked = 64 / kStaged;  // steps of a look-up
+        const auto token_of = [&](int step, int j) {
+            return begin + step * kStepTokens + key_wave * kTile + (column_wave * kStaged + j) * kKv8Granule;
+        };
+        Lookup looked{};
         auto load = [&](int step) {
-            const int first = begin + step * kTile + wave * kKv8Granule;
-            const int at = min(first, (end - 1) & ~(kKv8Granule - 1));
-            int page = table[at / kPage];
-            held = min(max(end - first, 0), kKv8Granule);
-            if (page < 0 || page >= p.cache.pages) page = 0, held = 0;
-            const size_t offset = page * page_bytes + at % kPage / kKv8Granule * kKv8GranuleBytes;
+            if (step % kLooked == 0) looked = look_up<kPage>(p, table, kv_head, token_of(step + lane / kStaged, lane % kStaged), end);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                k_bytes[c] = *reinterpret_cast<const uint4*>(keys + offset + c * 1024);
-                v_bytes[c] = *reinterpret_cast<const uint4*>(values + offset + c * 1024);
+            for (int j = 0; j < kStaged; ++j) {
+                const int from = step % kLooked * kStaged + j, first = token_of(step, j);
+                const int page = of_lane(looked.page, from);
+                const int at = min(first, (end - 1) & ~(kKv8Granule - 1));
+                held[j] = page < 0 ? 0 : min(max(end - first, 0), kKv8Granule);
+                const size_t offset = max(page, 0) * page_bytes + at % kPage / kKv8Granule * kKv8GranuleBytes;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    k_bytes[j][c] = *reinterpret_cast<const uint4*>(keys + offset + c * 1024);
+                    v_bytes[j][c] = *reinterpret_cast<const uint4*>(values + offset + c * 1024);
+                }
+                key_scale[j] = of_lane(looked.key_scale, from);
+                value_scale[j] = of_lane(looked.value_scale, from);
             }
-            const size_t scale_at = static_cast<size_t>(page) * p.cache.key_value_heads + kv_head;
-            key_scale = p.cache.key_scales[scale_at] * p.scale2;
-            value_scale = p.cache.value_scales[scale_at];
         };
         auto stage = [&](int buffer) {
-            // keys: lane (token, 16-dimension group): two 16-byte groups of bf16 for each half of the dimensions
-            const int token = wave * kKv8Granule + (lane >> 2);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const uint2 a = bf16_of<kFormat>(k_bytes[c].x), b = bf16_of<kFormat>(k_bytes[c].y);
-                const uint2 d = bf16_of<kFormat>(k_bytes[c].z), e = bf16_of<kFormat>(k_bytes[c].w);
-                const int group = 8 * c + 2 * (lane & 3);
-                *reinterpret_cast<uint4*>(&key_lds[buffer][token * 256 + (group ^ (token & 15)) * 16]) = uint4{a.x, a.y, b.x, b.y};
-                *reinterpret_cast<uint4*>(&key_lds[buffer][token * 256 + ((group + 1) ^ (token & 15)) * 16]) = uint4{d.x, d.y, e.x, e.y};
-            }
-            // values: lane (token / 4, d % 16): four tokens of dimensions 64 c + 16 t + d % 16
-            const unsigned mask = byte_mask(4 * (lane >> 4), 0, held);
-            const int place = 2 * wave + (lane >> 5);
+            for (int j = 0; j < kStaged; ++j) {
+                const int granule = column_wave * kStaged + j;
+                // keys: lane (token, 16-dimension group): two 16-byte groups of bf16 for each half of the dimensions
+                const int token = lane >> 2;
+                unsigned char* to = &lds.keys[buffer][key_wave][(granule * kKv8Granule + token) * 256];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const unsigned w[4] = {v_bytes[c].x, v_bytes[c].y, v_bytes[c].z, v_bytes[c].w};
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const int d = 64 * c + 16 * t + (lane & 15);
-                    *reinterpret_cast<uint2*>(&value_lds[buffer][d * 128 + (place ^ (d >> 1 & 7)) * 16 + (lane >> 4 & 1) * 8]) =
-                        bf16_of<kFormat>(w[t] & mask);
+                for (int c = 0; c < 2; ++c) {
+                    const uint2 a = bf16_of<kFormat>(k_bytes[j][c].x), b = bf16_of<kFormat>(k_bytes[j][c].y);
+                    const uint2 d = bf16_of<kFormat>(k_bytes[j][c].z), e = bf16_of<kFormat>(k_bytes[j][c].w);
+                    const int group = 8 * c + 2 * (lane & 3);
+                    *reinterpret_cast<uint4*>(to + (group ^ token) * 16) = uint4{a.x, a.y, b.x, b.y};
+                    *reinterpret_cast<uint4*>(to + ((group + 1) ^ token) * 16) = uint4{d.x, d.y, e.x, e.y};
                 }
-            }
-            if (lane == 0) {
-                key_scale_lds[buffer][wave] = held > 0 ? key_scale : 0.0f;
-                value_scale_lds[buffer][wave] = held > 0 ? value_scale : 0.0f;
-                held_lds[buffer][wave] = held;
+                // values: lane (token / 4, d % 16): four tokens of dimensions 64 c + 16 t + d % 16.  Their scale goes
+                // into the weights as a power, 2^(score + log2 scale); below kLeastScale the values take the rest of it,
+                // so that a page of tiny values does not push its weights, which the sum needs, out of fp32.
+                const float kept = fmaxf(value_scale[j], kLeastScale);
+                const int place = 2 * granule + (lane >> 5);
+                unsigned mask = 0xffffffffu;
+                if (held[j] < kKv8Granule) mask = byte_mask(4 * (lane >> 4), 0, held[j]);
+                const bool tiny = value_scale[j] < kLeastScale;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const unsigned w[4] = {v_bytes[j][c].x, v_bytes[j][c].y, v_bytes[j][c].z, v_bytes[j][c].w};
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const int d = 64 * c + 16 * t + (lane & 15);
+                        uint2 v = bf16_of<kFormat>(w[t] & mask);
+                        if (tiny) v = scaled_bf16_of<kFormat>(w[t] & mask, value_scale[j] * (1.0f / kLeastScale));
+                        *reinterpret_cast<uint2*>(&lds.values[buffer][key_wave][d * 128 + (place ^ (d >> 1 & 7)) * 16 + (lane >> 4 & 1) * 8]) = v;
+                    }
+                }
+                if (lane == 0) {
+                    const bool any = held[j] > 0;
+                    lds.key_scale[buffer][key_wave][granule] = any ? key_scale[j] : 0.0f;
+                    lds.value_log[buffer][key_wave][granule] = any ? __builtin_amdgcn_logf(kept) : 0.0f;
+                    lds.value_inverse[buffer][key_wave][granule] = any ? 1.0f / kept : 1.0f;
+                    lds.held[buffer][key_wave][granule] = held[j];
+                }
             }
         };
 
@@ -401,42 +518,31 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void kv8_many_rows_kernel(Param
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
-        if (steps > 0) load(0);
-        for (int step = 0; step < steps; ++step) {
-            const int buffer = step & 1;
-            stage(buffer);
-            if (step + 1 < steps) load(step + 1);
-            __syncthreads();
-            const int token0 = begin + step * kTile;
-            if (!wave_lives || token0 > wave_last || (p.a.window > 0 && token0 + kTile - 1 <= wave_first - p.a.window)) continue;
-            // row i of a 32-token tile is token i with bits 2 and 3 exchanged
-            const int token = (column & 19) | (column & 4) << 1 | (column & 8) >> 1;
+        // row i of a 32-token tile is token i with bits 2 and 3 exchanged
+        const int key_row = (column & 19) | (column & 4) << 1 | (column & 8) >> 1;
+        auto compute = [&](int buffer, int token0) {
             floatx16_t s[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
-                const unsigned char* from = &key_lds[buffer][(32 * t + token) * 256];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(from + ((2 * k + half) ^ (token & 15)) * 16);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[k], s[t], 0, 0, 0);
-                }
-            }
-            float factor[kTileGranules], value_factor[kTileGranules];
-            bool whole = token0 + kTile - 1 <= wave_first && (p.a.window == 0 || token0 > wave_last - p.a.window);
-#pragma unroll
-            for (int g = 0; g < kTileGranules; ++g) {
-                factor[g] = key_scale_lds[buffer][g];
-                value_factor[g] = value_scale_lds[buffer][g];
-                whole &= held_lds[buffer][g] == kKv8Granule;
-            }
-            // s[t][i]: token 32 t + 16 (i / 8) + 8 half + i % 8
-            float top = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[t][i] *= factor[2 * t + (i >> 3)];
+                for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const unsigned char* from = &lds.keys[buffer][key_wave][(32 * t + key_row) * 256];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(from + ((2 * k + half) ^ (key_row & 15)) * 16);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[k], s[t], 0, 0, 0);
+                }
+            }
+            float factor[kTileGranules];
+            bool whole = token0 + kTile - 1 <= wave_first && (p.a.window == 0 || token0 > wave_last - p.a.window);
+#pragma unroll
+            for (int g = 0; g < kTileGranules; ++g) {
+                factor[g] = lds.key_scale[buffer][key_wave][g];
+                whole &= lds.held[buffer][key_wave][g] == kKv8Granule;
+            }
+            // s[t][i]: token 32 t + 16 (i / 8) + 8 half + i % 8, in units of its granule's scale
             if (!__builtin_amdgcn_readfirstlane(whole)) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -444,14 +550,23 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void kv8_many_rows_kernel(Param
                     for (int i = 0; i < 16; ++i) {
                         const int of_granule = 8 * half + (i & 7);
                         const int at = token0 + 32 * t + 16 * (i >> 3) + of_granule;
-                        const bool counts = at <= position && at > lowest && of_granule < held_lds[buffer][2 * t + (i >> 3)];
+                        const bool counts = at <= position && at > lowest && of_granule < lds.held[buffer][key_wave][2 * t + (i >> 3)];
                         s[t][i] = counts ? s[t][i] : -INFINITY;
                     }
+#pragma unroll
+                for (int g = 0; g < kTileGranules; ++g) {
+                    // -infinity stays what it is: 0 * -infinity would not
+                    factor[g] = fmaxf(factor[g], 0x1p-126f);
+                }
             }
+            float top = -INFINITY;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int g = 0; g < kTileGranules; ++g) {
+                float most = s[g >> 1][8 * (g & 1)];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+                for (int i = 1; i < 8; ++i) most = fmaxf(most, s[g >> 1][8 * (g & 1) + i]);
+                top = fmaxf(top, most * factor[g]);
+            }
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             if (__any(top > maximum + kSlack)) {
                 const float next = fmaxf(maximum, top);
@@ -466,31 +581,92 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void kv8_many_rows_kernel(Param
             const float reference = maximum == -INFINITY ? 0.0f : maximum;
             bf16x8_t weights[4];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
+            for (int g = 0; g < kTileGranules; ++g) {
+                const float shift = lds.value_log[buffer][key_wave][g] - reference;
                 unsigned w[4];
+                float part = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float a = __builtin_amdgcn_exp2f(s[g >> 1][8 * (g & 1) + 2 * i] - reference);
-                    const float b = __builtin_amdgcn_exp2f(s[g >> 1][8 * (g & 1) + 2 * i + 1] - reference);
-                    sum += a + b;
-                    w[i] = pack_bf16(a * value_factor[g], b * value_factor[g]);
+                    const float a = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + 2 * i], factor[g], shift));
+                    const float b = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + 2 * i + 1], factor[g], shift));
+                    part += a;
+                    part += b;
+                    w[i] = pack_bf16(a, b);
                 }
+                sum = fmaf(part, lds.value_inverse[buffer][key_wave][g], sum);
                 weights[g] = __builtin_bit_cast(bf16x8_t, uint4{w[0], w[1], w[2], w[3]});
             }
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
                 const int dimension = 32 * d + column;
-                const unsigned char* from = &value_lds[buffer][dimension * 128];
+                const unsigned char* from = &lds.values[buffer][key_wave][dimension * 128];
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(from + ((2 * g + half) ^ (dimension >> 1 & 7)) * 16);
                     acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, weights[g], acc[d], 0, 0, 0);
                 }
             }
+        };
+        if (steps > 0) load(0);
+        for (int step = 0; step < steps; ++step) {
+            const int buffer = kBuffers == 2 ? step & 1 : 0;
+            stage(buffer);
+            if (step + 1 < steps) load(step + 1);
+            __syncthreads();
+            const int token0 = begin + step * kStepTokens + key_wave * kTile;
+            // nothing of this wave's rows lies before their window or behind their last position
+            if (wave_lives && token0 <= wave_last && (p.a.window == 0 || token0 + kTile - 1 > wave_first - p.a.window)) {
+                compute(buffer, token0);
+            }
+            if constexpr (kBuffers == 1) __syncthreads();
         }
-        __syncthreads();  // the next tile of rows stages into the buffers
+        __syncthreads();  // the buffers are free: for the key groups' results, for the next tile of rows
         sum += __shfl_xor(sum, 32, 64);
-        if (mine) {
+        if constexpr (kKeyWaves > 1) {
+            if (half == 0) lds.maximum[key_wave][column_wave][column] = maximum, lds.sum[key_wave][column_wave][column] = sum;
+            __syncthreads();
+            float top = lds.maximum[0][column_wave][column];
+#pragma unroll
+            for (int g = 1; g < kKeyWaves; ++g) top = fmaxf(top, lds.maximum[g][column_wave][column]);
+            const float reference = top == -INFINITY ? 0.0f : top;
+            sum = 0.0f;
+#pragma unroll
+            for (int g = 0; g < kKeyWaves; ++g) {
+                sum += lds.sum[g][column_wave][column] * __builtin_amdgcn_exp2f(lds.maximum[g][column_wave][column] - reference);
+            }
+            const float shrink = __builtin_amdgcn_exp2f(maximum - reference);
+            // a column wave's 16 KB of each key group but the first, lane by lane
+            float* place = reinterpret_cast<float*>(dynamic_lds) + lane * 4;
+            static_assert(sizeof(lds.keys) + sizeof(lds.values) >= (kKeyWaves - 1) * kColumnWaves * 64 * 64 * 4, "results fit");
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
+            if (key_wave > 0) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        *reinterpret_cast<floatx4_t*>(place + (((key_wave - 1) * kColumnWaves + column_wave) * 16 + d * 4 + i) * 256) =
+                            floatx4_t{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+                    }
+            }
+            __syncthreads();
+            if (key_wave == 0) {
+#pragma unroll
+                for (int g = 0; g < kKeyWaves - 1; ++g)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const floatx4_t o = *reinterpret_cast<const floatx4_t*>(place + ((g * kColumnWaves + column_wave) * 16 + d * 4 + i) * 256);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[d][4 * i + e] += o[e];
+                        }
+            }
+            __syncthreads();
+        }
+        if (mine && key_wave == 0) {
             const float inverse = sum > 0.0f ? 1.0f / sum : 0.0f;
             bf16_t* to = p.a.out + static_cast<size_t>(rows.first + row) * p.a.out_stride + head * kDim + 4 * half;
 #pragma unroll
@@ -505,23 +681,35 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void kv8_many_rows_kernel(Param
     }
 }
 
+template <int kFormat, int kPageGranules, int kColumnWaves, int kKeyWaves>
+hipError_t launch_many_rows(const Params& p, hipStream_t stream) {
+    const auto kernel = kv8_many_rows_kernel<kFormat, kPageGranules, kColumnWaves, kKeyWaves>;
+    static std::atomic<unsigned long long> prepared{0};
+    constexpr int kBytes = sizeof(ManyShared<kColumnWaves, kKeyWaves>);
+    if (const hipError_t st = set_dynamic_lds_once(prepared, reinterpret_cast<const void*>(kernel), kBytes); st != hipSuccess) return st;
+    const int pairs = std::min(p.a.max_rows, p.a.rows) * p.group;
+    const int tiles = std::min((pairs + 32 * kColumnWaves - 1) / (32 * kColumnWaves), 65535);
+    kernel<<<dim3(p.cache.key_value_heads, tiles, p.a.sequences), 64 * kColumnWaves * kKeyWaves, kBytes, stream>>>(p);
+    return hipGetLastError();
+}
+
 template <int kFormat, int kPageGranules>
 hipError_t launch_pages(const Params& p, hipStream_t stream) {
-    const bool many = p.few != INT_MAX;
+    const bool many = p.many != kNone;
     if (!many || p.a.sequences > 1) {
-        kv8_few_rows_kernel<kFormat, kPageGranules>
-            <<<dim3(p.cache.key_value_heads, p.splits, p.a.sequences), 64 * kWaves, 0, stream>>>(p);
+        const dim3 grid(p.cache.key_value_heads, p.splits, p.a.sequences);
+        if (p.waves == 1) kv8_few_rows_kernel<kFormat, kPageGranules, 1><<<grid, 64, 0, stream>>>(p);
+        else kv8_few_rows_kernel<kFormat, kPageGranules, kFewWaves><<<grid, 64 * kFewWaves, 0, stream>>>(p);
         if (p.splits > 1) {
-            kv8_join_kernel<<<dim3(p.cache.key_value_heads, p.a.sequences), 64 * kWaves, 0, stream>>>(p);
+            kv8_join_kernel<<<dim3(p.columns, p.cache.key_value_heads, p.a.sequences), 32 * kJoinGroups, 0, stream>>>(p);
         }
     }
-    if (many) {
-        const int pairs = std::min(p.a.max_rows, p.a.rows) * p.group;
-        const int tiles = (pairs + 127) / 128;
-        kv8_many_rows_kernel<kFormat, kPageGranules, 4>
-            <<<dim3(p.cache.key_value_heads, std::min(tiles, 65535), p.a.sequences), 256, 0, stream>>>(p);
+    if (!many) return hipGetLastError();
+    switch (p.many) {
+        case kWide: return launch_many_rows<kFormat, kPageGranules, 4, 1>(p, stream);
+        case kHalved: return launch_many_rows<kFormat, kPageGranules, 4, 2>(p, stream);
+        default: return launch_many_rows<kFormat, kPageGranules, 2, 4>(p, stream);
     }
-    return hipGetLastError();
 }
 
 template <int kFormat>
@@ -535,24 +723,46 @@ hipError_t launch_format(const Params& p, hipStream_t stream) {
 
 // How a call's work is dealt out.
 struct Dealt {
-    bool many;    // sequences of many rows may be among them
-    int columns;  // as in Params
-    int splits;
+    int many = kNone;  // where sequences of many rows may be among them
+    int columns = 0;   // as in Params
+    int splits = 1;
+    int waves = kFewWaves;
 };
 constexpr int kBytesOfPartial = (kDim + 2) * 4;
+
 Dealt dealt_of(const Kv8Cache& cache, const Kv8AttentionArgs& a, size_t workspace_bytes) {
     Dealt d;
     const int group = a.query_heads / cache.key_value_heads;
     const int rows = std::max(1, std::min(a.max_rows, a.rows));
-    d.many = static_cast<long long>(rows) * group > 16;
+    const int reach = static_cast<int>(std::min<long long>(a.window > 0 ? static_cast<long long>(a.window) + rows : INT_MAX, a.max_length));
     d.columns = std::min(16 / group, rows) * group;
-    // Contexts are shared until two workgroups a CU are there, each with a step for every wave
+    if (static_cast<long long>(rows) * group > 16) {
+        // Blocks of 128 columns while two a CU are there, or where a chain of
+        // steps is short anyway; else the tokens of a step are dealt to two or
+        // four key groups, for the chain's sake.  One layer, 16 / 8 heads, us
+        // with 1 / 2 / 4 groups: prompts of 128 rows 10.1 / 10.9 / 11.9, 512
+        // 21.0 / 18.3 / 16.1, 1024 34.8 / 28.0 / 23.6, 2048 63 / 48 / 49, 4096
+        // 122 / 98 / 151; four prompts of 512 26.4 / 23.8 / 34.4, of 2048 120 /
+        // 121 / 191.
+        const long long blocks = static_cast<long long>(a.rows) * a.query_heads / 128;
+        d.many = blocks > 512 || reach <= 192 ? kWide : blocks <= 128 && reach >= 384 ? kQuartered : kHalved;
+        if (a.sequences == 1) return d;  // one prompt: no sequence of few rows
+    }
+    // Contexts are shared among workgroups until there is one a CU, or two
+    // where a workgroup would have more than 4096 tokens: then lengths differ
+    // most (16 sequences of 100..16000 tokens, two splits 72 us, four 62; 32 of
+    // 1000, one 15.8, two 18.9; one of 65521, 32 splits 28.5, 64 32.0).  A share
+    // is a step of every wave at least.
     const long long blocks = static_cast<long long>(std::max(a.sequences, 1)) * cache.key_value_heads;
-    const int reach = a.window > 0 ? std::min(a.window + rows, a.max_length) : a.max_length;
-    const long long wanted = std::min<long long>((512 + blocks - 1) / blocks, (reach + kWaves * kStep - 1) / (kWaves * kStep));
+    const auto for_blocks = [&](long long n) { return (n + blocks - 1) / blocks; };
+    const auto for_tokens = [&](int n) { return (static_cast<long long>(reach) + n - 1) / n; };
+    const long long wanted = std::max(for_blocks(256), std::min(for_blocks(512), for_tokens(4096)));
     const long long fits = static_cast<long long>(workspace_bytes / (static_cast<size_t>(blocks) * d.columns * kBytesOfPartial));
-    d.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({wanted, fits, 64})));
-    if (d.many && a.sequences == 1) d.splits = 1;  // one prompt: no sequence of few rows
+    d.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({wanted, for_tokens(kFewWaves * kStep), fits, 64})));
+    // Short contexts of many sequences: a wave a workgroup, none waits at the
+    // end for waves that had no step (256 sequences of 100 tokens 24.9 us, now
+    // 15.7; of 1111..8192 tokens 445, a wave each 499).
+    if (reach <= 512 && blocks >= 1024) d.waves = 1;
     return d;
 }
 
@@ -588,11 +798,14 @@ hipError_t launch_kv8_attention(const Kv8Cache& cache, const Kv8AttentionArgs& a
     p.a = a;
     p.cache = cache;
     p.group = a.query_heads / cache.key_value_heads;
-    p.scale2 = a.scale * kLog2E;
+    p.scale2 = std::fabs(a.scale) * kLog2E;
+    p.flip = a.scale < 0 ? 0x80008000u : 0u;
     const Dealt d = dealt_of(cache, a, a.workspace_bytes);
     p.columns = d.columns;
     p.splits = d.splits;
-    p.few = !d.many ? INT_MAX : a.sequences > 1 ? 16 : 0;
+    p.waves = d.waves;
+    p.many = d.many;
+    p.few = d.many == kNone ? INT_MAX : a.sequences > 1 ? 16 : 0;
     const size_t slots = static_cast<size_t>(a.sequences) * cache.key_value_heads * d.columns * d.splits;
     p.partial_out = a.workspace;
     p.partial_sums = reinterpret_cast<float2*>(a.workspace + slots * kDim);

@@ -382,13 +382,15 @@ def test_attention_single_tokens(hip, fmt, page, heads, kv_heads):
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("page", [16, 32, 64])
 @pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 3), (7, 1), (16, 1)])
-def test_attention_prompts(hip, fmt, page, heads, kv_heads):
-    """Whole prompts, chunks behind a context, single tokens and idle sequences together."""
+@pytest.mark.parametrize("max_length", [100, 300, 4096])
+def test_attention_prompts(hip, fmt, page, heads, kv_heads, max_length):
+    """Whole prompts, chunks behind a context, single tokens and idle sequences together; the length that the caller
+    names has the work dealt out in three ways."""
     rng = np.random.default_rng(heads * page + 1)
     lengths = [1, 40, 130, 300, 77, 0, 65, 200]
     new = [1, 40, 130, 33, 1, 0, 2, 17]
     store = Store(hip, fmt, page, sum(-(-l // page) for l in lengths) + 2, kv_heads, rng)
-    attend(hip, store, lengths, new, heads)
+    attend(hip, store, lengths, new, heads, max_length=max_length)
 
 
 @pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 65, 100, 1000])
