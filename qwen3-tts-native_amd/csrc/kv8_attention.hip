@@ -362,7 +362,9 @@ __global__ __launch_bounds__(32 * kJoinGroups) void kv8_join_kernel(Params p) {
 // ---------------------------------------------------------------------------
 constexpr int kTile = 64;  // tokens of a wave's step
 constexpr int kTileGranules = kTile / kKv8Granule;
-constexpr int kTileBytes = kTile * kDim * 2;  // as bf16
+// Rows of a tile in LDS, as bf16: 16 bytes of padding put the rows that 16 lanes
+// read at once in different banks, and leave one address for all of a lane's reads.
+constexpr int kKeyRow = kDim * 2 + 16, kValueRow = kTile * 2 + 16;
 // a maximum may stay this far (log2) behind the scores before the sums are scaled anew
 constexpr float kSlack = 8.0f;
 // Smallest value scale that goes into the weights as it is, see stage().
@@ -379,8 +381,8 @@ __device__ __forceinline__ uint2 scaled_bf16_of(unsigned w, float factor) {
 template <int kColumnWaves, int kKeyWaves>
 struct ManyShared {
     static constexpr int kBuffers = kKeyWaves == 1 ? 2 : 1;
-    unsigned char keys[kBuffers][kKeyWaves][kTileBytes];    // [token][16-byte groups of dimensions, swizzled]
-    unsigned char values[kBuffers][kKeyWaves][kTileBytes];  // [dimension][16-byte groups of tokens, swizzled]
+    unsigned char keys[kBuffers][kKeyWaves][kTile * kKeyRow];    // [token][dimension]
+    unsigned char values[kBuffers][kKeyWaves][kDim * kValueRow];  // [dimension][token]
     float key_scale[kBuffers][kKeyWaves][kTileGranules];
     float value_log[kBuffers][kKeyWaves][kTileGranules];      // log2 of the values' scale
     float value_inverse[kBuffers][kKeyWaves][kTileGranules];  // and its reciprocal
@@ -474,32 +476,38 @@ __global__ __launch_bounds__(64 * kColumnWaves * kKeyWaves, 2) void kv8_many_row
                 const int granule = column_wave * kStaged + j;
                 // keys: lane (token, 16-dimension group): two 16-byte groups of bf16 for each half of the dimensions
                 const int token = lane >> 2;
-                unsigned char* to = &lds.keys[buffer][key_wave][(granule * kKv8Granule + token) * 256];
+                unsigned char* to = &lds.keys[buffer][key_wave][(granule * kKv8Granule + token) * kKeyRow + (lane & 3) * 32];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const uint2 a = bf16_of<kFormat>(k_bytes[j][c].x), b = bf16_of<kFormat>(k_bytes[j][c].y);
                     const uint2 d = bf16_of<kFormat>(k_bytes[j][c].z), e = bf16_of<kFormat>(k_bytes[j][c].w);
-                    const int group = 8 * c + 2 * (lane & 3);
-                    *reinterpret_cast<uint4*>(to + (group ^ token) * 16) = uint4{a.x, a.y, b.x, b.y};
-                    *reinterpret_cast<uint4*>(to + ((group + 1) ^ token) * 16) = uint4{d.x, d.y, e.x, e.y};
+                    *reinterpret_cast<uint4*>(to + c * 128) = uint4{a.x, a.y, b.x, b.y};
+                    *reinterpret_cast<uint4*>(to + c * 128 + 16) = uint4{d.x, d.y, e.x, e.y};
                 }
                 // values: lane (token / 4, d % 16): four tokens of dimensions 64 c + 16 t + d % 16.  Their scale goes
                 // into the weights as a power, 2^(score + log2 scale); below kLeastScale the values take the rest of it,
                 // so that a page of tiny values does not push its weights, which the sum needs, out of fp32.
                 const float kept = fmaxf(value_scale[j], kLeastScale);
-                const int place = 2 * granule + (lane >> 5);
+                unsigned char* values_to = &lds.values[buffer][key_wave][(lane & 15) * kValueRow + granule * 32 + (lane >> 4) * 8];
                 unsigned mask = 0xffffffffu;
                 if (held[j] < kKv8Granule) mask = byte_mask(4 * (lane >> 4), 0, held[j]);
-                const bool tiny = value_scale[j] < kLeastScale;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const unsigned w[4] = {v_bytes[j][c].x, v_bytes[j][c].y, v_bytes[j][c].z, v_bytes[j][c].w};
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
-                        const int d = 64 * c + 16 * t + (lane & 15);
-                        uint2 v = bf16_of<kFormat>(w[t] & mask);
-                        if (tiny) v = scaled_bf16_of<kFormat>(w[t] & mask, value_scale[j] * (1.0f / kLeastScale));
-                        *reinterpret_cast<uint2*>(&lds.values[buffer][key_wave][d * 128 + (place ^ (d >> 1 & 7)) * 16 + (lane >> 4 & 1) * 8]) = v;
+                        *reinterpret_cast<uint2*>(values_to + (64 * c + 16 * t) * kValueRow) = bf16_of<kFormat>(w[t] & mask);
+                    }
+                }
+                if (value_scale[j] < kLeastScale) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const unsigned w[4] = {v_bytes[j][c].x, v_bytes[j][c].y, v_bytes[j][c].z, v_bytes[j][c].w};
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            *reinterpret_cast<uint2*>(values_to + (64 * c + 16 * t) * kValueRow) =
+                                scaled_bf16_of<kFormat>(w[t] & mask, value_scale[j] * (1.0f / kLeastScale));
+                        }
                     }
                 }
                 if (lane == 0) {
@@ -521,20 +529,27 @@ __global__ __launch_bounds__(64 * kColumnWaves * kKeyWaves, 2) void kv8_many_row
         // row i of a 32-token tile is token i with bits 2 and 3 exchanged
         const int key_row = (column & 19) | (column & 4) << 1 | (column & 8) >> 1;
         auto compute = [&](int buffer, int token0) {
+            const unsigned char* keys_from = &lds.keys[buffer][key_wave][key_row * kKeyRow + half * 16];
+            const unsigned char* values_from = &lds.values[buffer][key_wave][column * kValueRow + half * 16];
+            bf16x8_t fragment[16];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) fragment[2 * k + t] = *reinterpret_cast<const bf16x8_t*>(keys_from + 32 * t * kKeyRow + 32 * k);
             floatx16_t s[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const unsigned char* from = &lds.keys[buffer][key_wave][(32 * t + key_row) * 256];
+            for (int k = 0; k < 8; ++k)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(from + ((2 * k + half) ^ (key_row & 15)) * 16);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[k], s[t], 0, 0, 0);
-                }
-            }
+                for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fragment[2 * k + t], q[k], s[t], 0, 0, 0);
+            bf16x8_t value[16];
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) value[4 * d + g] = *reinterpret_cast<const bf16x8_t*>(values_from + 32 * d * kValueRow + 32 * g);
             float factor[kTileGranules];
             bool whole = token0 + kTile - 1 <= wave_first && (p.a.window == 0 || token0 > wave_last - p.a.window);
 #pragma unroll
@@ -597,15 +612,15 @@ __global__ __launch_bounds__(64 * kColumnWaves * kKeyWaves, 2) void kv8_many_row
                 weights[g] = __builtin_bit_cast(bf16x8_t, uint4{w[0], w[1], w[2], w[3]});
             }
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                const int dimension = 32 * d + column;
-                const unsigned char* from = &lds.values[buffer][key_wave][dimension * 128];
+            for (int d = 2; d < 4; ++d)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(from + ((2 * g + half) ^ (dimension >> 1 & 7)) * 16);
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, weights[g], acc[d], 0, 0, 0);
-                }
-            }
+                for (int g = 0; g < 4; ++g) value[4 * d + g] = *reinterpret_cast<const bf16x8_t*>(values_from + 32 * d * kValueRow + 32 * g);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int d = e; d < e + 2; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value[4 * d + g], weights[g], acc[d], 0, 0, 0);
         };
         if (steps > 0) load(0);
         for (int step = 0; step < steps; ++step) {
