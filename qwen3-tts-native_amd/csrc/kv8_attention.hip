@@ -100,16 +100,21 @@ __device__ __forceinline__ float of_lane(float v, int lane) {
 constexpr int kStep = 64;  // tokens of a wave's step
 constexpr int kStepGranules = kStep / kKv8Granule;
 
+template <int kWaves>
+struct FewShared {
+    __align__(16) float out[kWaves][8 * 64 * 4];
+    float maximum[kWaves][16], sum[kWaves][16];
+};
+
 template <int kFormat, int kPageGranules, int kWaves>
-// Two waves a SIMD: with registers for three (168) the compiler spills, and
-// 256 sequences up to 8192 tokens take 601 us instead of 445.
-__global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) {
-    __shared__ __align__(16) float out_lds[kWaves][8 * 64 * 4];
-    __shared__ float max_lds[kWaves][16], sum_lds[kWaves][16];
+__device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds, int split) {
+    auto& out_lds = lds.out;
+    auto& max_lds = lds.maximum;
+    auto& sum_lds = lds.sum;
     constexpr int kPage = kPageGranules * kKv8Granule;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int column = lane & 15, quad = lane >> 4;
-    const int kv_head = blockIdx.x, split = blockIdx.y, sequence = blockIdx.z;
+    const int kv_head = blockIdx.x, sequence = blockIdx.z;
     const Rows rows = rows_of(p, sequence);
     const int splits = splits_of(p, rows);
     if (split >= splits) return;
@@ -304,6 +309,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) 
     }
 }
 
+// Two waves a SIMD: with registers for three (168) the compiler spills, and
+// 256 sequences up to 8192 tokens take 601 us instead of 445.
+template <int kFormat, int kPageGranules, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 2) void kv8_few_rows_kernel(Params p) {
+    __shared__ FewShared<kWaves> lds;
+    few_rows<kFormat, kPageGranules, kWaves>(p, lds, blockIdx.y);
+}
+
 // Joins the results of workgroups that shared a context: a workgroup a (row,
 // head), its 8 groups of 32 lanes take every eighth of the partial results
 // (one wave for all of them: 18 us for 64 of a row, now 4).
@@ -391,9 +404,8 @@ struct ManyShared {
 };
 
 template <int kFormat, int kPageGranules, int kColumnWaves, int kKeyWaves>
-__global__ __launch_bounds__(64 * kColumnWaves * kKeyWaves, 2) void kv8_many_rows_kernel(Params p) {
+__device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynamic_lds, int first_tile, int tiles_apart) {
     using Shared = ManyShared<kColumnWaves, kKeyWaves>;
-    extern __shared__ __align__(16) unsigned char dynamic_lds[];
     Shared& lds = *reinterpret_cast<Shared*>(dynamic_lds);
     constexpr int kBuffers = Shared::kBuffers;
     constexpr int kPage = kPageGranules * kKv8Granule;
@@ -415,7 +427,7 @@ __global__ __launch_bounds__(64 * kColumnWaves * kKeyWaves, 2) void kv8_many_row
     const int tiles = (pairs + kColumns - 1) / kColumns;
 
     // the longest rows first: they are the launch's tail
-    for (int tile = tiles - 1 - static_cast<int>(blockIdx.y); tile >= 0; tile -= gridDim.y) {
+    for (int tile = tiles - 1 - first_tile; tile >= 0; tile -= tiles_apart) {
         const int pair = tile * kColumns + column_wave * 32 + column;
         const bool mine = pair < pairs;
         const int row = min(pair, pairs - 1) / p.group;
@@ -696,35 +708,54 @@ __global__ __launch_bounds__(64 * kColumnWaves * kKeyWaves, 2) void kv8_many_row
     }
 }
 
+// Sequences of few rows and of many in one launch, so that neither waits for
+// the other's last workgroup: workgroups y < splits take the former's shares,
+// the others the latter's tiles; a sequence has one of the two.  Sequence after
+// sequence, and heads side by side: with eight key/value heads each XCD's L2
+// holds one head of one sequence at a time (every sequence's longest tiles
+// first instead, four prompts of 1777..4096 rows 363 -> 555 us).
 template <int kFormat, int kPageGranules, int kColumnWaves, int kKeyWaves>
-hipError_t launch_many_rows(const Params& p, hipStream_t stream) {
-    const auto kernel = kv8_many_rows_kernel<kFormat, kPageGranules, kColumnWaves, kKeyWaves>;
+__global__ __launch_bounds__(64 * kColumnWaves * kKeyWaves, 2) void kv8_all_rows_kernel(Params p) {
+    constexpr int kWaves = kColumnWaves * kKeyWaves;
+    extern __shared__ __align__(16) unsigned char dynamic_lds[];
+    const int shares = p.few > 0 ? p.splits : 0, y = blockIdx.y;
+    if (y < shares) {
+        few_rows<kFormat, kPageGranules, kWaves>(p, *reinterpret_cast<FewShared<kWaves>*>(dynamic_lds), y);
+    } else {
+        many_rows<kFormat, kPageGranules, kColumnWaves, kKeyWaves>(p, dynamic_lds, y - shares, gridDim.y - shares);
+    }
+}
+
+template <int kFormat, int kPageGranules, int kColumnWaves, int kKeyWaves>
+hipError_t launch_all_rows(const Params& p, hipStream_t stream) {
+    const auto kernel = kv8_all_rows_kernel<kFormat, kPageGranules, kColumnWaves, kKeyWaves>;
     static std::atomic<unsigned long long> prepared{0};
-    constexpr int kBytes = sizeof(ManyShared<kColumnWaves, kKeyWaves>);
+    constexpr int kWaves = kColumnWaves * kKeyWaves;
+    constexpr int kBytes = std::max(sizeof(ManyShared<kColumnWaves, kKeyWaves>), sizeof(FewShared<kWaves>));
     if (const hipError_t st = set_dynamic_lds_once(prepared, reinterpret_cast<const void*>(kernel), kBytes); st != hipSuccess) return st;
-    const int pairs = std::min(p.a.max_rows, p.a.rows) * p.group;
-    const int tiles = std::min((pairs + 32 * kColumnWaves - 1) / (32 * kColumnWaves), 65535);
-    kernel<<<dim3(p.cache.key_value_heads, tiles, p.a.sequences), 64 * kColumnWaves * kKeyWaves, kBytes, stream>>>(p);
+    const int pairs = std::min(p.a.max_rows, p.a.rows) * p.group, shares = p.few > 0 ? p.splits : 0;
+    const int tiles = std::min((pairs + 32 * kColumnWaves - 1) / (32 * kColumnWaves), 65535 - shares);
+    kernel<<<dim3(p.cache.key_value_heads, shares + tiles, p.a.sequences), 64 * kWaves, kBytes, stream>>>(p);
     return hipGetLastError();
 }
 
 template <int kFormat, int kPageGranules>
 hipError_t launch_pages(const Params& p, hipStream_t stream) {
-    const bool many = p.many != kNone;
-    if (!many || p.a.sequences > 1) {
-        const dim3 grid(p.cache.key_value_heads, p.splits, p.a.sequences);
-        if (p.waves == 1) kv8_few_rows_kernel<kFormat, kPageGranules, 1><<<grid, 64, 0, stream>>>(p);
-        else kv8_few_rows_kernel<kFormat, kPageGranules, kFewWaves><<<grid, 64 * kFewWaves, 0, stream>>>(p);
-        if (p.splits > 1) {
-            kv8_join_kernel<<<dim3(p.columns, p.cache.key_value_heads, p.a.sequences), 32 * kJoinGroups, 0, stream>>>(p);
-        }
-    }
-    if (!many) return hipGetLastError();
+    const dim3 grid(p.cache.key_value_heads, p.splits, p.a.sequences);
+    hipError_t st = hipSuccess;
     switch (p.many) {
-        case kWide: return launch_many_rows<kFormat, kPageGranules, 4, 1>(p, stream);
-        case kHalved: return launch_many_rows<kFormat, kPageGranules, 4, 2>(p, stream);
-        default: return launch_many_rows<kFormat, kPageGranules, 2, 4>(p, stream);
+        case kNone:
+            if (p.waves == 1) kv8_few_rows_kernel<kFormat, kPageGranules, 1><<<grid, 64, 0, stream>>>(p);
+            else kv8_few_rows_kernel<kFormat, kPageGranules, kFewWaves><<<grid, 64 * kFewWaves, 0, stream>>>(p);
+            st = hipGetLastError();
+            break;
+        case kWide: st = launch_all_rows<kFormat, kPageGranules, 4, 1>(p, stream); break;
+        case kHalved: st = launch_all_rows<kFormat, kPageGranules, 4, 2>(p, stream); break;
+        default: st = launch_all_rows<kFormat, kPageGranules, 2, 4>(p, stream); break;
     }
+    if (st != hipSuccess || p.splits == 1) return st;
+    kv8_join_kernel<<<dim3(p.columns, p.cache.key_value_heads, p.a.sequences), 32 * kJoinGroups, 0, stream>>>(p);
+    return hipGetLastError();
 }
 
 template <int kFormat>
