@@ -602,7 +602,8 @@ QWEN3_TTS_API int32_t qwen3_tts_op_kv8_append_v1(
  * most 16 of them share one.  Rows that no sequence has are left as they were; a row
  * with nothing to attend to becomes 0, and a table entry that is no page
  * counts as nothing.  query and out are bf16 [rows][stride] (strides in
- * elements, multiples of 8 and 4; 16- and 8-byte aligned) and may be the same.
+ * elements, multiples of 8 and 4; 16- and 8-byte aligned) and may be the same
+ * buffer with the same stride.  Scales of the cache are not negative.
  * max_rows and max_length are what the caller knows of the largest sequence's
  * rows and length (the graph's, where it is captured): they choose how the work is
  * dealt out, results hold beyond them.  workspace is scratch for sharing long

@@ -232,7 +232,7 @@ def test_append_in_pieces(hip, fmt, page, heads):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
-@pytest.mark.parametrize("page,rows,heads", [(16, 700, 8), (32, 1111, 5), (64, 900, 8)])
+@pytest.mark.parametrize("page,rows,heads", [(16, 700, 8), (32, 1111, 5), (64, 900, 8), (16, 2900, 8), (64, 2500, 8)])
 def test_append_many_rows(hip, fmt, page, rows, heads):
     """Many sequences' rows at once, runs that begin anywhere, rows left out between them."""
     rng = np.random.default_rng(rows)
@@ -401,6 +401,28 @@ def test_attention_window(hip, window, many):
     new = [1, 60, 65, 70, 1] if many else [1, 1, 3, 2, 1]
     store = Store(hip, "int8" if window % 2 else "e4m3", 32, 25, 2, rng)
     attend(hip, store, lengths, new, 4, window=window)
+
+
+@pytest.mark.parametrize("fmt,page", [("int8", 16), ("e4m3", 32), ("int8", 64)])
+def test_attention_many_short_sequences(hip, fmt, page):
+    """A wave a workgroup: many sequences of contexts up to 110 tokens."""
+    rng = np.random.default_rng(page + 50)
+    lengths = [int(l) for l in rng.integers(0, 111, 140)]
+    new = [int(l > 0 and rng.random() < 0.9) for l in lengths]
+    store = Store(hip, fmt, page, sum(-(-l // page) for l in lengths) + 2, 8, rng)
+    attend(hip, store, lengths, new, 16)
+
+
+def test_attention_shared_prefix(hip):
+    """Two sequences whose tables name the same pages."""
+    rng = np.random.default_rng(51)
+    store = Store(hip, "int8", 16, 26, 2, rng)
+
+    def spoil(tables):
+        tables[1, :10] = tables[0, :10]
+
+    for new in ([1, 1], [70, 90]):
+        attend(hip, store, [200, 175], new, 4, spoil=spoil)
 
 
 @pytest.mark.parametrize("workspace", [0, 1 << 12, 1 << 16, 1 << 24])
@@ -620,6 +642,75 @@ def test_steps_captured_into_a_graph(hip):
     finally:
         rt.destroy(graph, exe)
         hip.load().qwen3_tts_stream_destroy(s)
+
+
+def test_steps_with_the_decode_primitives(hip):
+    """A decode step as a model makes it: the plan's positions rotate the normalized query and key heads, which the
+    append stores and the attention reads."""
+    rng = np.random.default_rng(31)
+    heads, kv_heads, sequences, pages = 4, 2, 5, 30
+    plan = Plan(hip, 16, pages, np.full((sequences, 8), -1, np.int32), np.zeros(sequences, int), rng.permutation(pages),
+                pages, 64, in_place=True)
+    store = Store(hip, "int8", 16, pages, kv_heads)
+    gains = [dev(hip, gen.gains(rng, D)) for _ in range(2)]
+    lengths = np.zeros(sequences, int)
+    for _ in range(6):
+        new = traffic(rng, lengths, 14)
+        want = plan.expected(new)
+        q, k, v = (kv_rows(rng, 64, h, spread=False) for h in (heads, kv_heads, kv_heads))
+        dq, dk, dv, out = dev(hip, q), dev(hip, k), dev(hip, v), dev(hip, np.zeros((64, heads * D), np.uint16))
+        plan.new_tokens.upload(np.array(new, np.int32))
+        plan.launch()
+        for array, n, gain in ((dq, heads, gains[0]), (dk, kv_heads, gains[1])):
+            hip.call("qwen3_tts_op_head_rms_norm_rows", array.ptr, gain.ptr, 64, n, D, C.c_float(1e-6), None)
+            hip.call("qwen3_tts_op_rope_rows", array.ptr, 64, n, D, plan.row_positions.ptr, C.c_float(1e6), None)
+        hip.kv8_append(store.cache, dk, dv, plan.row_slots, 64)
+        hip.kv8_attention(store.cache, dq, out, heads, 64, sequences, plan.tables, plan.stride, plan.new_lengths,
+                          plan.row_starts, max_rows=14, max_length=128)
+        hip.synchronize()
+        plan.check(want)
+        live, lengths = int(want["row_starts"][-1]), want["new_lengths"]
+        store.append(dk.numpy(), v, want["row_slots"])
+        ref, tolerance = model.attention("int8", 16, *store.codes, *store.scales, gen.f32(dq.numpy()), want["tables"],
+                                         lengths, want["row_starts"], heads, D ** -0.5, 0, MANY_ROWS)
+        off = np.abs(gen.f32(out.numpy())[:live].reshape(live, heads, D) - ref[:live])
+        assert np.all(off <= tolerance[:live])
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = {paths!r}
+import numpy as np
+import qwen3_tts_hip as hip
+import test_kv8_gpu as t
+from test_zz_no_alloc import Runtime
+hip.load()
+rt, rng = Runtime(hip), np.random.default_rng(3)
+server = t.Server(hip, rng, "int8", 16, 4, 40, 300, 4, 2)
+s = rt.stream()
+graph, exe = rt.capture(s, lambda: server.launch(s))
+
+def replay():
+    rt.launch(exe, s)
+    rt.sync(s)
+
+lengths = np.zeros(4, int)
+for new in ([200, 0, 30, 1], [1, 17, 1, 1], [-1, 1, 1, 1], [260, 1, 1, -1]):
+    lengths = server.step(rng, new, replay)["new_lengths"]
+print("same after capture as the first call")
+"""
+
+
+def test_first_calls_of_a_process_under_capture(hip):
+    """A fresh process whose first launches of the three operators are captured; every replay is right."""
+    import pathlib
+    import subprocess
+    import sys
+
+    here = pathlib.Path(__file__).resolve().parent
+    paths = [str(here), str(here.parent / "qwen3-tts-native_amd")]
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL.format(paths=paths)], capture_output=True, text=True, timeout=100)
+    assert run.returncode == 0 and "same after capture" in run.stdout, run.stdout + run.stderr
 
 
 def test_two_streams_with_workspaces_of_their_own(hip):
