@@ -404,15 +404,19 @@ __device__ __forceinline__ uint2 scaled_bf16_of(unsigned w, float factor) {
                  pack_bf16(__uint_as_float(v.y << 16) * factor, __uint_as_float(v.y & 0xffff0000u) * factor)};
 }
 
+// What a step has to know of a granule: the keys' scale times the scores', log2
+// of the values' scale and its reciprocal, tokens that hold something.
+struct __align__(16) Granule {
+    float key_scale, value_log, value_inverse;
+    int held;
+};
+
 template <int kColumnWaves, int kKeyWaves>
 struct ManyShared {
     static constexpr int kBuffers = kKeyWaves == 1 ? 2 : 1;
     unsigned char keys[kBuffers][kKeyWaves][kTile * kKeyRow];    // [token][dimension]
     unsigned char values[kBuffers][kKeyWaves][kDim * kValueRow];  // [dimension][token]
-    float key_scale[kBuffers][kKeyWaves][kTileGranules];
-    float value_log[kBuffers][kKeyWaves][kTileGranules];      // log2 of the values' scale
-    float value_inverse[kBuffers][kKeyWaves][kTileGranules];  // and its reciprocal
-    int held[kBuffers][kKeyWaves][kTileGranules];
+    Granule granules[kBuffers][kKeyWaves][kTileGranules];
     float maximum[kKeyWaves][kColumnWaves][32], sum[kKeyWaves][kColumnWaves][32];
 };
 
@@ -470,28 +474,37 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
         const int wave_last = rows.position + min(wave_pair + 31, pairs - 1) / p.group;
 
         uint4 k_bytes[kStaged][2], v_bytes[kStaged][2];
-        float key_scale[kStaged], value_scale[kStaged];
-        int held[kStaged];
+        Granule staged[kStaged];
+        float value_scale[kStaged];
         constexpr int kLooked = 64 / kStaged;  // steps of a look-up
         const auto token_of = [&](int step, int j) {
             return begin + step * kStepTokens + key_wave * kTile + (column_wave * kStaged + j) * kKv8Granule;
         };
         Lookup looked{};
+        float looked_log = 0.0f, looked_inverse = 1.0f;
         auto load = [&](int step) {
-            if (step % kLooked == 0) looked = look_up<kPage>(p, table, kv_head, token_of(step + lane / kStaged, lane % kStaged), end);
+            if (step % kLooked == 0) {
+                looked = look_up<kPage>(p, table, kv_head, token_of(step + lane / kStaged, lane % kStaged), end);
+                // Values' scale goes into the weights as a power, 2^(score + log2 scale); below kLeastScale the values
+                // take the rest of it, so that a page of tiny values does not push its weights, which the sum
+                // needs, out of fp32.
+                const float kept = fmaxf(looked.value_scale, kLeastScale);
+                looked_log = __builtin_amdgcn_logf(kept);
+                looked_inverse = 1.0f / kept;
+            }
 #pragma unroll
             for (int j = 0; j < kStaged; ++j) {
                 const int from = step % kLooked * kStaged + j, first = token_of(step, j);
                 const int page = of_lane(looked.page, from);
                 const int at = min(first, (end - 1) & ~(kKv8Granule - 1));
-                held[j] = page < 0 ? 0 : min(max(end - first, 0), kKv8Granule);
                 const size_t offset = max(page, 0) * page_bytes + at % kPage / kKv8Granule * kKv8GranuleBytes;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     k_bytes[j][c] = *reinterpret_cast<const uint4*>(keys + offset + c * 1024);
                     v_bytes[j][c] = *reinterpret_cast<const uint4*>(values + offset + c * 1024);
                 }
-                key_scale[j] = of_lane(looked.key_scale, from);
+                staged[j] = Granule{of_lane(looked.key_scale, from), of_lane(looked_log, from), of_lane(looked_inverse, from),
+                                    page < 0 ? 0 : min(max(end - first, 0), kKv8Granule)};
                 value_scale[j] = of_lane(looked.value_scale, from);
             }
         };
@@ -509,13 +522,10 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
                     *reinterpret_cast<uint4*>(to + c * 128) = uint4{a.x, a.y, b.x, b.y};
                     *reinterpret_cast<uint4*>(to + c * 128 + 16) = uint4{d.x, d.y, e.x, e.y};
                 }
-                // values: lane (token / 4, d % 16): four tokens of dimensions 64 c + 16 t + d % 16.  Their scale goes
-                // into the weights as a power, 2^(score + log2 scale); below kLeastScale the values take the rest of it,
-                // so that a page of tiny values does not push its weights, which the sum needs, out of fp32.
-                const float kept = fmaxf(value_scale[j], kLeastScale);
+                // values: lane (token / 4, d % 16): four tokens of dimensions 64 c + 16 t + d % 16
                 unsigned char* values_to = &lds.values[buffer][key_wave][(lane & 15) * kValueRow + granule * 32 + (lane >> 4) * 8];
                 unsigned mask = 0xffffffffu;
-                if (held[j] < kKv8Granule) mask = byte_mask(4 * (lane >> 4), 0, held[j]);
+                if (staged[j].held < kKv8Granule) mask = byte_mask(4 * (lane >> 4), 0, staged[j].held);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const unsigned w[4] = {v_bytes[j][c].x, v_bytes[j][c].y, v_bytes[j][c].z, v_bytes[j][c].w};
@@ -535,13 +545,7 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
                         }
                     }
                 }
-                if (lane == 0) {
-                    const bool any = held[j] > 0;
-                    lds.key_scale[buffer][key_wave][granule] = any ? key_scale[j] : 0.0f;
-                    lds.value_log[buffer][key_wave][granule] = any ? __builtin_amdgcn_logf(kept) : 0.0f;
-                    lds.value_inverse[buffer][key_wave][granule] = any ? 1.0f / kept : 1.0f;
-                    lds.held[buffer][key_wave][granule] = held[j];
-                }
+                if (lane == 0) lds.granules[buffer][key_wave][granule] = staged[j];
             }
         };
 
@@ -575,28 +579,30 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
             for (int d = 0; d < 2; ++d)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) value[4 * d + g] = *reinterpret_cast<const bf16x8_t*>(values_from + 32 * d * kValueRow + 32 * g);
-            float factor[kTileGranules];
+            Granule of[kTileGranules];
             bool whole = token0 + kTile - 1 <= wave_first && (p.a.window == 0 || token0 > wave_last - p.a.window);
 #pragma unroll
             for (int g = 0; g < kTileGranules; ++g) {
-                factor[g] = lds.key_scale[buffer][key_wave][g];
-                whole &= lds.held[buffer][key_wave][g] == kKv8Granule;
+                of[g] = lds.granules[buffer][key_wave][g];
+                whole &= of[g].held == kKv8Granule;
             }
             // s[t][i]: token 32 t + 16 (i / 8) + 8 half + i % 8, in units of its granule's scale
             if (!__builtin_amdgcn_readfirstlane(whole)) {
+                // kept a branch: the compiler would fold its 160 operations into every step
+                asm volatile("");
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int of_granule = 8 * half + (i & 7);
                         const int at = token0 + 32 * t + 16 * (i >> 3) + of_granule;
-                        const bool counts = at <= position && at > lowest && of_granule < lds.held[buffer][key_wave][2 * t + (i >> 3)];
+                        const bool counts = at <= position && at > lowest && of_granule < of[2 * t + (i >> 3)].held;
                         s[t][i] = counts ? s[t][i] : -INFINITY;
                     }
 #pragma unroll
                 for (int g = 0; g < kTileGranules; ++g) {
                     // -infinity stays what it is: 0 * -infinity would not
-                    factor[g] = fmaxf(factor[g], 0x1p-126f);
+                    of[g].key_scale = fmaxf(of[g].key_scale, 0x1p-126f);
                 }
             }
             float top = -INFINITY;
@@ -605,7 +611,7 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
                 float most = s[g >> 1][8 * (g & 1)];
 #pragma unroll
                 for (int i = 1; i < 8; ++i) most = fmaxf(most, s[g >> 1][8 * (g & 1) + i]);
-                top = fmaxf(top, most * factor[g]);
+                top = fmaxf(top, most * of[g].key_scale);
             }
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             if (__any(top > maximum + kSlack)) {
@@ -622,18 +628,18 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
             bf16x8_t weights[4];
 #pragma unroll
             for (int g = 0; g < kTileGranules; ++g) {
-                const float shift = lds.value_log[buffer][key_wave][g] - reference;
+                const float shift = of[g].value_log - reference;
                 unsigned w[4];
                 float part = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float a = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + 2 * i], factor[g], shift));
-                    const float b = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + 2 * i + 1], factor[g], shift));
+                    const float a = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + 2 * i], of[g].key_scale, shift));
+                    const float b = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + 2 * i + 1], of[g].key_scale, shift));
                     part += a;
                     part += b;
                     w[i] = pack_bf16(a, b);
                 }
-                sum = fmaf(part, lds.value_inverse[buffer][key_wave][g], sum);
+                sum = fmaf(part, of[g].value_inverse, sum);
                 weights[g] = __builtin_bit_cast(bf16x8_t, uint4{w[0], w[1], w[2], w[3]});
             }
 #pragma unroll
