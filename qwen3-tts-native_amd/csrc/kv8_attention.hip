@@ -380,10 +380,10 @@ __global__ __launch_bounds__(32 * kJoinGroups) void kv8_join_kernel(Params p) {
 // product O^T = V^T P^T: weights never leave their lane.
 // Waves are kColumnWaves x kKeyWaves: those of a key group take the same 64 of
 // every 64 * kKeyWaves tokens, and the groups' results are joined at the end.
-// Prompts of 1777..4096 rows, 32 / 8 heads: 361 us, 851 TFLOP/s (the library's
+// Prompts of 1777..4096 rows, 32 / 8 heads: 361 us, 850 TFLOP/s (the library's
 // large product reaches 1213); one of 801 rows, 16 / 8 heads: 22 us, latency.
-// Two waves a SIMD share the matrix cores (32 % busy), the vector unit (42 %) and
-// LDS (about 40 %), none of them full: leaving out the exponentials, the
+// Two waves a SIMD share the matrix cores (40 % of a busy CU's time), the vector
+// unit (52 %) and LDS (40 %), none of them full: leaving out the exponentials, the
 // value products, the staging or the loads saves 6 to 12 % each.
 // ---------------------------------------------------------------------------
 constexpr int kTile = 64;  // tokens of a wave's step
