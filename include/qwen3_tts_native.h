@@ -547,7 +547,8 @@ typedef struct Qwen3TtsKv8CacheV1 {
  * new_lengths may be lengths and new_free_count may be free_count; other
  * buffers must not overlap.  A page may stand in several tables (a shared
  * prefix) while no sequence writes to it or ends: giving back a page twice
- * puts it on the stack twice. */
+ * puts it on the stack twice, and an entry that is no page is given back as it
+ * is. */
 typedef struct Qwen3TtsKv8PlanV1 {
     uint32_t struct_size;
     int32_t sequences;
@@ -601,7 +602,8 @@ QWEN3_TTS_API int32_t qwen3_tts_op_kv8_append_v1(
  * query head h reads key/value head h / (query_heads / key_value_heads), at
  * most 16 of them share one.  Rows that no sequence has are left as they were; a row
  * with nothing to attend to becomes 0, and a table entry that is no page
- * counts as nothing.  query and out are bf16 [rows][stride] (strides in
+ * counts as nothing.  Tokens that no row attends to, in front of a window or
+ * behind a length, are not looked at as numbers: their entries may be stale.  query and out are bf16 [rows][stride] (strides in
  * elements, multiples of 8 and 4; 16- and 8-byte aligned) and may be the same
  * buffer with the same stride.  Scales of the cache are not negative.
  * max_rows and max_length are what the caller knows of the largest sequence's

@@ -78,14 +78,16 @@ struct Lookup {
     int page;  // -1: none
     float key_scale, value_scale;
 };
-// `token` is the first of the lane's granule, `end` the end of what counts.
+// `token` is the first of the lane's granule; tokens [low, end) are those that
+// any of the rows attends to.  Nothing else of a sequence is looked at as a
+// number: pages in front of a window may have been given to others.
 template <int kPage>
-__device__ __forceinline__ Lookup look_up(const Params& p, const int* table, int kv_head, int token, int end) {
+__device__ __forceinline__ Lookup look_up(const Params& p, const int* table, int kv_head, int token, int low, int end) {
     const int at = min(token, (end - 1) & ~(kKv8Granule - 1));  // past the end: the last one again
     int page = table[at / kPage];
     if (page < 0 || page >= p.cache.pages) page = -1;
     const size_t scale_at = static_cast<size_t>(max(page, 0)) * p.cache.key_value_heads + kv_head;
-    const bool counts = page >= 0 && token < end;
+    const bool counts = page >= 0 && token < end && token + kKv8Granule > low;
     return Lookup{page, counts ? p.cache.key_scales[scale_at] * p.scale2 : 0.0f, counts ? p.cache.value_scales[scale_at] : 0.0f};
 }
 __device__ __forceinline__ int of_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
@@ -157,7 +159,8 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
         // tokens [begin, end) of this tile's rows, in steps dealt to the splits, then to the waves
         const int last = min(tile + rows_per_tile, rows.count) - 1;
         const int end = min(rows.position + last + 1, rows.length);
-        const int begin = p.a.window > 0 ? max(rows.position + tile - p.a.window + 1, 0) & ~(kStep - 1) : 0;
+        const int low = p.a.window > 0 ? max(rows.position + tile - p.a.window + 1, 0) : 0;
+        const int begin = low & ~(kStep - 1);
         const int steps = end > begin ? (end - begin + kStep - 1) / kStep : 0;
         const int share = (steps + splits - 1) / splits;
         const int steps_begin = split * share, steps_end = min(steps_begin + share, steps);
@@ -175,7 +178,7 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
         uint4 k[kStepGranules][2], v[kStepGranules][2];
         Lookup looked{};
         const auto look = [&](int i) {
-            looked = look_up<kPage>(p, table, kv_head, token_of(i + lane / kStepGranules) + lane % kStepGranules * kKv8Granule, end);
+            looked = look_up<kPage>(p, table, kv_head, token_of(i + lane / kStepGranules) + lane % kStepGranules * kKv8Granule, low, end);
         };
         const auto offset_of = [&](int i, int g) {
             const int page = max(of_lane(looked.page, i % kLooked * kStepGranules + g), 0);
@@ -237,7 +240,7 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
 #pragma unroll
             for (int d = 0; d < 8; ++d) acc[d] *= shrink;
             // weights times the values' scale as two bf16, the second what the first leaves: 16 bits of them
-            unsigned high[kStepGranules][2], low[kStepGranules][2];
+            unsigned high[kStepGranules][2], rest[kStepGranules][2];
 #pragma unroll
             for (int g = 0; g < kStepGranules; ++g) {
                 float w[4];
@@ -250,12 +253,13 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     high[g][e] = pack_bf16(w[2 * e], w[2 * e + 1]);
-                    low[g][e] = pack_bf16(w[2 * e] - __uint_as_float(high[g][e] << 16),
-                                          w[2 * e + 1] - __uint_as_float(high[g][e] & 0xffff0000u));
+                    rest[g][e] = pack_bf16(w[2 * e] - __uint_as_float(high[g][e] << 16),
+                                           w[2 * e + 1] - __uint_as_float(high[g][e] & 0xffff0000u));
                 }
-                if (held[g] < kKv8Granule) {
-                    // bytes behind the length may hold anything, an e4m3 NaN too, which a zero weight would not silence
-                    const unsigned mask = byte_mask(4 * quad, 0, held[g]);
+                const int skipped = low - token0 - g * kKv8Granule;
+                if (held[g] < kKv8Granule || skipped > 0) {
+                    // bytes that do not count may hold anything, an e4m3 NaN too, which a zero weight would not silence
+                    const unsigned mask = byte_mask(4 * quad, skipped, held[g]);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) v[g][c] = uint4{v[g][c].x & mask, v[g][c].y & mask, v[g][c].z & mask, v[g][c].w & mask};
                 }
@@ -263,7 +267,7 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
 #pragma unroll
             for (int g = 0; g < kStepGranules; g += 2) {
                 const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, uint4{high[g][0], high[g][1], high[g + 1][0], high[g + 1][1]});
-                const bf16x8_t pl = __builtin_bit_cast(bf16x8_t, uint4{low[g][0], low[g][1], low[g + 1][0], low[g + 1][1]});
+                const bf16x8_t pl = __builtin_bit_cast(bf16x8_t, uint4{rest[g][0], rest[g][1], rest[g + 1][0], rest[g + 1][1]});
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const unsigned a[4] = {v[g][c].x, v[g][c].y, v[g][c].z, v[g][c].w};
@@ -466,7 +470,8 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
         const int first_row = tile * kColumns / p.group;
         const int last_row = min(tile * kColumns + kColumns - 1, pairs - 1) / p.group;
         const int end = min(rows.position + last_row + 1, rows.length);
-        const int begin = p.a.window > 0 ? max(rows.position + first_row - p.a.window + 1, 0) & ~(kTile - 1) : 0;
+        const int low = p.a.window > 0 ? max(rows.position + first_row - p.a.window + 1, 0) : 0;
+        const int begin = low & ~(kTile - 1);
         const int steps = end > begin ? (end - begin + kStepTokens - 1) / kStepTokens : 0;
         const int wave_pair = tile * kColumns + column_wave * 32;
         const bool wave_lives = wave_pair < pairs;
@@ -476,6 +481,7 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
         uint4 k_bytes[kStaged][2], v_bytes[kStaged][2];
         Granule staged[kStaged];
         float value_scale[kStaged];
+        int skipped[kStaged];  // tokens of the granule in front of every row's window
         constexpr int kLooked = 64 / kStaged;  // steps of a look-up
         const auto token_of = [&](int step, int j) {
             return begin + step * kStepTokens + key_wave * kTile + (column_wave * kStaged + j) * kKv8Granule;
@@ -484,7 +490,7 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
         float looked_log = 0.0f, looked_inverse = 1.0f;
         auto load = [&](int step) {
             if (step % kLooked == 0) {
-                looked = look_up<kPage>(p, table, kv_head, token_of(step + lane / kStaged, lane % kStaged), end);
+                looked = look_up<kPage>(p, table, kv_head, token_of(step + lane / kStaged, lane % kStaged), low, end);
                 // Values' scale goes into the weights as a power, 2^(score + log2 scale); below kLeastScale the values
                 // take the rest of it, so that a page of tiny values does not push its weights, which the sum
                 // needs, out of fp32.
@@ -506,6 +512,7 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
                 staged[j] = Granule{of_lane(looked.key_scale, from), of_lane(looked_log, from), of_lane(looked_inverse, from),
                                     page < 0 ? 0 : min(max(end - first, 0), kKv8Granule)};
                 value_scale[j] = of_lane(looked.value_scale, from);
+                skipped[j] = low - first;
             }
         };
         auto stage = [&](int buffer) {
@@ -525,7 +532,7 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
                 // values: lane (token / 4, d % 16): four tokens of dimensions 64 c + 16 t + d % 16
                 unsigned char* values_to = &lds.values[buffer][key_wave][(lane & 15) * kValueRow + granule * 32 + (lane >> 4) * 8];
                 unsigned mask = 0xffffffffu;
-                if (staged[j].held < kKv8Granule) mask = byte_mask(4 * (lane >> 4), 0, staged[j].held);
+                if (staged[j].held < kKv8Granule || skipped[j] > 0) mask = byte_mask(4 * (lane >> 4), skipped[j], staged[j].held);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const unsigned w[4] = {v_bytes[j][c].x, v_bytes[j][c].y, v_bytes[j][c].z, v_bytes[j][c].w};

@@ -403,6 +403,33 @@ def test_attention_window(hip, window, many):
     attend(hip, store, lengths, new, 4, window=window)
 
 
+@pytest.mark.parametrize("fmt,page", [("e4m3", 16), ("int8", 16), ("e4m3", 64)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [1, 90, 60]])
+def test_attention_window_over_stale_pages(hip, fmt, page, new):
+    """Pages in front of every row's window were given away: their bytes and scales are no numbers, or their entries
+    no pages."""
+    rng = np.random.default_rng(page + 60)
+    window, lengths = 45, [300, 299, 170]
+    store = Store(hip, fmt, page, 60, 2, rng)
+
+    def spoil(tables):
+        stale = []
+        for s, (length, n) in enumerate(zip(lengths, new)):
+            low = max(length - n - window + 1, 0)
+            for at in range(low // page):
+                stale.append(int(tables[s, at]))
+                if at % 3 == 0:
+                    tables[s, at] = -7
+        assert stale
+        for i, is_key in enumerate((True, False)):
+            raw, scales = store.raw[i].numpy(), store.device_scales[i].numpy()
+            raw[stale], scales[stale] = model.NAN_BYTE[fmt], np.nan
+            store.raw[i].upload(raw)
+            store.device_scales[i].upload(scales)
+
+    attend(hip, store, lengths, new, 4, window=window, spoil=spoil)
+
+
 @pytest.mark.parametrize("fmt,page", [("int8", 16), ("e4m3", 32), ("int8", 64)])
 def test_attention_many_short_sequences(hip, fmt, page):
     """A wave a workgroup: many sequences of contexts up to 110 tokens."""
