@@ -40,6 +40,7 @@ struct Params {
     int waves = kFewWaves;  // of a workgroup of few rows
     int many = kNone;
     int few = INT_MAX;  // pairs up to which a sequence counts as one of few rows
+    int few_tiles = 1;  // workgroups among which the tiles of its rows are dealt
     float* partial_out = nullptr;   // [sequence][kv head][column][split][128]
     float2* partial_sums = nullptr;  // [sequence][kv head][column][split] (maximum, sum)
 };
@@ -117,7 +118,7 @@ struct FewShared {
 };
 
 template <int kFormat, int kPageGranules, int kWaves>
-__device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds, int split) {
+__device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds, int share) {
     auto& out_lds = lds.out;
     auto& max_lds = lds.maximum;
     auto& sum_lds = lds.sum;
@@ -127,6 +128,8 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
     const int kv_head = blockIdx.x, sequence = blockIdx.z;
     const Rows rows = rows_of(p, sequence);
     const int splits = splits_of(p, rows);
+    const int split = share / p.few_tiles;
+    const int first_tile = p.few_tiles - 1 - share % p.few_tiles;  // a prompt's longest first
     if (split >= splits) return;
     const int rows_per_tile = 16 / p.group;
     const int head = kv_head * p.group + column % p.group;
@@ -137,7 +140,7 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
     const unsigned char* keys_of_lane = p.cache.key_pages + kv_head * (kPageGranules * kKv8GranuleBytes) +
                                         (lane & 15) * 64 + quad * 16;
 
-    for (int tile = 0; tile < rows.count; tile += rows_per_tile) {
+    for (int tile = first_tile * rows_per_tile; tile < rows.count; tile += p.few_tiles * rows_per_tile) {
         const int row = tile + column / p.group;
         const bool mine = column < rows_per_tile * p.group && row < rows.count;
         const int position = mine ? rows.position + row : -1;
@@ -162,8 +165,8 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
         const int low = p.a.window > 0 ? max(rows.position + tile - p.a.window + 1, 0) : 0;
         const int begin = low & ~(kStep - 1);
         const int steps = end > begin ? (end - begin + kStep - 1) / kStep : 0;
-        const int share = (steps + splits - 1) / splits;
-        const int steps_begin = split * share, steps_end = min(steps_begin + share, steps);
+        const int steps_each = (steps + splits - 1) / splits;
+        const int steps_begin = split * steps_each, steps_end = min(steps_begin + steps_each, steps);
         const int lowest = p.a.window > 0 ? position - p.a.window : -1;  // tokens above it count
 
         float maximum = -INFINITY, sum = 0.0f;
@@ -300,7 +303,7 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
         __syncthreads();
         // wave w: dimension tiles of 16, every column
         if (mine) {
-            const size_t slot = partial_slot(p, sequence, kv_head, column) + split;
+            const size_t slot = partial_slot(p, sequence, kv_head, tile * p.group + column) + split;
 #pragma unroll
             for (int j = 0; j < 8 / kWaves; ++j) {
                 const int d = 8 / kWaves * wave + j;
@@ -744,7 +747,7 @@ template <int kFormat, int kPageGranules, int kColumnWaves, int kKeyWaves>
 __global__ __launch_bounds__(64 * kColumnWaves * kKeyWaves, 2) void kv8_all_rows_kernel(Params p) {
     constexpr int kWaves = kColumnWaves * kKeyWaves;
     extern __shared__ __align__(16) unsigned char dynamic_lds[];
-    const int shares = p.few > 0 ? p.splits : 0, y = blockIdx.y;
+    const int shares = p.few > 0 ? p.splits * p.few_tiles : 0, y = blockIdx.y;
     if (y < shares) {
         few_rows<kFormat, kPageGranules, kWaves>(p, *reinterpret_cast<FewShared<kWaves>*>(dynamic_lds), y);
     } else {
@@ -759,7 +762,7 @@ hipError_t launch_all_rows(const Params& p, hipStream_t stream) {
     constexpr int kWaves = kColumnWaves * kKeyWaves;
     constexpr int kBytes = std::max(sizeof(ManyShared<kColumnWaves, kKeyWaves>), sizeof(FewShared<kWaves>));
     if (const hipError_t st = set_dynamic_lds_once(prepared, reinterpret_cast<const void*>(kernel), kBytes); st != hipSuccess) return st;
-    const int pairs = std::min(p.a.max_rows, p.a.rows) * p.group, shares = p.few > 0 ? p.splits : 0;
+    const int pairs = std::min(p.a.max_rows, p.a.rows) * p.group, shares = p.few > 0 ? p.splits * p.few_tiles : 0;
     const int tiles = std::min((pairs + 32 * kColumnWaves - 1) / (32 * kColumnWaves), 65535 - shares);
     kernel<<<dim3(p.cache.key_value_heads, shares + tiles, p.a.sequences), 64 * kWaves, kBytes, stream>>>(p);
     return hipGetLastError();
@@ -767,7 +770,7 @@ hipError_t launch_all_rows(const Params& p, hipStream_t stream) {
 
 template <int kFormat, int kPageGranules>
 hipError_t launch_pages(const Params& p, hipStream_t stream) {
-    const dim3 grid(p.cache.key_value_heads, p.splits, p.a.sequences);
+    const dim3 grid(p.cache.key_value_heads, p.splits * p.few_tiles, p.a.sequences);
     hipError_t st = hipSuccess;
     switch (p.many) {
         case kNone:
@@ -796,7 +799,7 @@ hipError_t launch_format(const Params& p, hipStream_t stream) {
 // How a call's work is dealt out.
 struct Dealt {
     int many = kNone;  // where sequences of many rows may be among them
-    int columns = 0;   // as in Params
+    int few = INT_MAX, columns = 0, few_tiles = 1;  // as in Params
     int splits = 1;
     int waves = kFewWaves;
 };
@@ -807,34 +810,62 @@ Dealt dealt_of(const Kv8Cache& cache, const Kv8AttentionArgs& a, size_t workspac
     const int group = a.query_heads / cache.key_value_heads;
     const int rows = std::max(1, std::min(a.max_rows, a.rows));
     const int reach = static_cast<int>(std::min<long long>(a.window > 0 ? static_cast<long long>(a.window) + rows : INT_MAX, a.max_length));
-    d.columns = std::min(16 / group, rows) * group;
-    if (static_cast<long long>(rows) * group > 16) {
-        // Blocks of 128 columns while two a CU are there, or where a chain of
+    const long long blocks = static_cast<long long>(std::max(a.sequences, 1)) * cache.key_value_heads;
+    const int tile = 16 / group;  // rows of a tile of few rows
+    const long long pairs = static_cast<long long>(rows) * group;
+    const auto tiles_of = [&](long long n) { return static_cast<int>((n / group + tile - 1) / tile); };
+    // Tiles of 16 pairs and blocks of 128 that the rows make at least, and the
+    // tokens that a row attends to on average where all lengths are the longest.
+    const long long few_tiles = std::max(blocks, static_cast<long long>(a.rows) * a.query_heads / 16);
+    const long long many_blocks = std::max(blocks, static_cast<long long>(a.rows) * a.query_heads / 128);
+    const auto tokens_of = [&](int tile_rows) -> double {
+        return a.window > 0 ? std::min<long long>(static_cast<long long>(a.window) + tile_rows, reach) : reach - std::min(rows, reach) / 2;
+    };
+    const double chain = a.window > 0 ? tokens_of(128 / group) : reach;
+    // All rows in tiles of 16, whose shares fill the chip, or in blocks of 128,
+    // which read and convert keys and values once for all columns?  us, fitted to
+    // one layer of 1 to 100 sequences: tiles 6.5 and 1 for each 33000 tokens of a
+    // tile, which has 120 more to start; blocks 11 and the longer of a chain, 0.0116 a
+    // token, and of the whole chip's work, 0.08 for 1000 tokens of a block.  Measured,
+    // 16 / 8 heads, blocks / tiles: 32 rows over 4000 tokens 56 / 13, 256 over 16000
+    // 197 / 117, 512 over 16000 197 / 217; prompts of 256 rows 13.0 / 6.9, 801 22.3 / 20.8,
+    // 1024 23.9 / 25.1; eight sequences' 128 over 4000 70 / 112; forty's 16 over 2000
+    // 113 / 57.  Not where most sequences would find no tile of theirs.
+    const bool tiles_win = few_tiles * (tokens_of(tile) + 120) / 33000 < 4.5 + std::max(0.0116 * chain, 8e-5 * many_blocks * tokens_of(128 / group));
+    if (pairs <= 16 || (tiles_win && blocks * tiles_of(pairs) <= 4 * few_tiles + 1024)) {
+        d.columns = static_cast<int>(pairs);
+    } else {
+        // Blocks of 128 columns where that makes one a CU, or where a chain of
         // steps is short anyway; else the tokens of a step are dealt to two or
         // four key groups, for the chain's sake.  One layer, 16 / 8 heads, us
-        // with 1 / 2 / 4 groups: prompts of 128 rows 10.1 / 10.9 / 11.9, 512
-        // 21.0 / 18.3 / 16.1, 1024 34.8 / 28.0 / 23.6, 2048 63 / 48 / 49, 4096
-        // 122 / 98 / 151; four prompts of 512 26.4 / 23.8 / 34.4, of 2048 120 /
-        // 121 / 191.
-        const long long blocks = static_cast<long long>(a.rows) * a.query_heads / 128;
-        d.many = blocks > 512 || reach <= 192 ? kWide : blocks <= 128 && reach >= 384 ? kQuartered : kHalved;
-        if (a.sequences == 1) return d;  // one prompt: no sequence of few rows
+        // with 1 / 2 / 4 groups: prompts of 512 rows 20.4 / 18.3 / 16.5, 1024 33.8 /
+        // 28.0 / 23.5, 2048 62 / 48 / 48, 4096 119 / 98 / 139; four prompts of 512 25.7
+        // / 23.7 / 36.0, of 801 40.7 / 43.0 / 59.6, of 2048 118 / 121 / 182.
+        const bool one = a.sequences == 1;
+        d.many = many_blocks > (one ? 512 : 256) || reach <= 192 ? kWide
+                 : many_blocks <= 128 && reach >= 384            ? kQuartered
+                                                                 : kHalved;
+        // sequences of few rows among them: up to two tiles, four while those are not many
+        d.few = one ? 0 : blocks <= 64 ? 64 : 32;
+        if (one) return d;
+        d.columns = static_cast<int>(std::min<long long>(d.few / group, rows)) * group;
     }
+    d.few_tiles = d.many == kNone ? tiles_of(d.columns) : 1;
     // Contexts are shared among workgroups until there is one a CU, or two
     // where a workgroup would have more than 4096 tokens: then lengths differ
     // most (16 sequences of 100..16000 tokens, two splits 72 us, four 62; 32 of
     // 1000, one 15.8, two 18.9; one of 65521, 32 splits 28.5, 64 32.0).  A share
     // is a step of every wave at least.
-    const long long blocks = static_cast<long long>(std::max(a.sequences, 1)) * cache.key_value_heads;
-    const auto for_blocks = [&](long long n) { return (n + blocks - 1) / blocks; };
+    const long long there = d.many == kNone ? std::min(blocks * d.few_tiles, few_tiles) : blocks;
+    const auto for_blocks = [&](long long n) { return (n + there - 1) / there; };
     const auto for_tokens = [&](int n) { return (static_cast<long long>(reach) + n - 1) / n; };
     const long long wanted = std::max(for_blocks(256), std::min(for_blocks(512), for_tokens(4096)));
     const long long fits = static_cast<long long>(workspace_bytes / (static_cast<size_t>(blocks) * d.columns * kBytesOfPartial));
-    d.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({wanted, for_tokens(kFewWaves * kStep), fits, 64})));
+    d.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({wanted, for_tokens(kFewWaves * kStep), fits, 64, 65535 / d.few_tiles})));
     // Short contexts of many sequences: a wave a workgroup, none waits at the
     // end for waves that had no step (256 sequences of 100 tokens 24.9 us, now
     // 15.7; of 1111..8192 tokens 445, a wave each 499).
-    if (reach <= 512 && blocks >= 1024) d.waves = 1;
+    if (reach <= 512 && there >= 1024) d.waves = 1;
     return d;
 }
 
@@ -877,7 +908,8 @@ hipError_t launch_kv8_attention(const Kv8Cache& cache, const Kv8AttentionArgs& a
     p.splits = d.splits;
     p.waves = d.waves;
     p.many = d.many;
-    p.few = d.many == kNone ? INT_MAX : a.sequences > 1 ? 16 : 0;
+    p.few = d.few;
+    p.few_tiles = d.few_tiles;
     const size_t slots = static_cast<size_t>(a.sequences) * cache.key_value_heads * d.columns * d.splits;
     p.partial_out = a.workspace;
     p.partial_sums = reinterpret_cast<float2*>(a.workspace + slots * kDim);

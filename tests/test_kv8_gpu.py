@@ -313,8 +313,9 @@ def test_append_strided_rows(hip):
 # Attention
 # ---------------------------------------------------------------------------
 def attend(hip, store, lengths, new, heads, *, window=0, scale=D ** -0.5, seed=0, workspace=0, max_rows=None,
-           max_length=None, spoil=None, tail_rows=3, query_pad=0, out_pad=0, sharp=1.0):
-    """One attention over `lengths` tokens and `new` rows a sequence; compares all rows, and those behind the last."""
+           max_length=None, spoil=None, tail_rows=3, query_pad=0, out_pad=0, sharp=1.0, few=None):
+    """One attention over `lengths` tokens and `new` rows a sequence; compares all rows, and those behind the last.
+    `few` says which products compute them, where a name of more rows than there are makes that other than it seems."""
     rng = np.random.default_rng(seed)
     page, sequences = store.page, len(lengths)
     count = [-(-l // page) for l in lengths]
@@ -353,7 +354,7 @@ def attend(hip, store, lengths, new, heads, *, window=0, scale=D ** -0.5, seed=0
     hip.synchronize()
     got = out.numpy()
     group = heads // store.heads
-    few = max(new) * group <= 16
+    few = max(new) * group <= 16 if few is None else few
     want, tolerance = model.attention(store.fmt, page, *store.codes, *store.scales, gen.f32(q[:, :width]), tables,
                                       lengths, starts, heads, scale, window, FEW_ROWS if few else MANY_ROWS)
     live = int(starts[-1])
@@ -532,6 +533,132 @@ def test_attention_in_place(hip):
             hip.synchronize()
             outs.append(out.numpy())
         assert np.array_equal(outs[0], outs[1])
+
+
+# Few rows are dealt out in tiles of 16 pairs, many in blocks of 128 columns whose waves share the columns (wide), or
+# the columns and the tokens (halved, quartered).  The rows that the buffers hold, used or not, and the sizes that the
+# caller names choose among them: buffers of so many tiles of 16 pairs take each.
+BLOCKS = {"wide": 2100, "halved": 1400, "quartered": 780}
+
+
+def in_blocks(kind, heads):
+    return {"tail_rows": BLOCKS[kind] * 16 // heads, "max_length": 4096}
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 3), (7, 1), (16, 1)])
+@pytest.mark.parametrize("kind", BLOCKS)
+def test_attention_prompts_in_blocks(hip, fmt, page, heads, kv_heads, kind):
+    rng = np.random.default_rng(heads * page + 2)
+    lengths = [1, 40, 130, 300, 77, 0, 65, 200]
+    new = [1, 40, 130, 33, 1, 0, 2, 17]
+    store = Store(hip, fmt, page, sum(-(-l // page) for l in lengths) + 2, kv_heads, rng)
+    attend(hip, store, lengths, new, heads, **in_blocks(kind, heads))
+
+
+@pytest.mark.parametrize("kind", BLOCKS)
+@pytest.mark.parametrize("length,rows", [(1, 1), (33, 33), (1000, 700), (700, 129)])
+def test_attention_one_prompt_in_blocks(hip, kind, length, rows):
+    rng = np.random.default_rng(length)
+    store = Store(hip, "int8", 16, 70, 2, rng)
+    attend(hip, store, [length], [rows], 4, max_rows=700, few=False, **in_blocks(kind, 4))
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 65, 100, 1000])
+@pytest.mark.parametrize("kind", BLOCKS)
+def test_attention_window_in_blocks(hip, window, kind):
+    rng = np.random.default_rng(window + 1)
+    lengths = [1, 64, 65, 300, 129]
+    store = Store(hip, "int8" if window % 2 else "e4m3", 32, 25, 2, rng)
+    attend(hip, store, lengths, [1, 60, 65, 70, 1], 4, window=window, max_rows=400, **in_blocks(kind, 4))
+
+
+@pytest.mark.parametrize("fmt,page", [("e4m3", 16), ("int8", 16), ("e4m3", 64)])
+@pytest.mark.parametrize("kind", BLOCKS)
+def test_attention_window_over_stale_pages_in_blocks(hip, fmt, page, kind):
+    rng = np.random.default_rng(page + 70)
+    window, lengths, new = 200, [500, 499, 370], [1, 90, 60]
+    store = Store(hip, fmt, page, 100, 2, rng)
+
+    def spoil(tables):
+        stale = []
+        for s, (length, n) in enumerate(zip(lengths, new)):
+            for at in range(max(length - n - window + 1, 0) // page):
+                stale.append(int(tables[s, at]))
+                if at % 3 == 0:
+                    tables[s, at] = -7
+        assert stale
+        for i in (0, 1):
+            raw, scales = store.raw[i].numpy(), store.device_scales[i].numpy()
+            raw[stale], scales[stale] = model.NAN_BYTE[fmt], np.nan
+            store.raw[i].upload(raw)
+            store.device_scales[i].upload(scales)
+
+    attend(hip, store, lengths, new, 4, window=window, spoil=spoil, max_rows=400, **in_blocks(kind, 4))
+
+
+@pytest.mark.parametrize("workspace", [0, 1 << 12, 1 << 16, 1 << 24])
+@pytest.mark.parametrize("new", [[31, 9, 1], [8, 32, 33], [500, 1, 20]])
+@pytest.mark.parametrize("kind", [None, *BLOCKS])
+def test_attention_long_context_of_some_rows(hip, workspace, new, kind):
+    """Sequences of one to four tiles, alone or beside longer ones."""
+    rng = np.random.default_rng(18)
+    store = Store(hip, "e4m3", 16, 420, 1, rng)
+    more = in_blocks(kind, 2) if kind else {}
+    attend(hip, store, [5000, 900, 64], new, 2, workspace=workspace, **more)
+
+
+@pytest.mark.parametrize("kind", BLOCKS)
+def test_attention_of_odd_numbers_in_blocks(hip, kind):
+    """Strides, scales, scores far apart, pages of unequal scales, tables that share pages or name none."""
+    rng = np.random.default_rng(19)
+    more = in_blocks(kind, 4)
+    store = Store(hip, "int8", 16, 60, 2, rng)
+    attend(hip, store, [400, 99], [90, 3], 4, query_pad=8 * D, out_pad=4, scale=-0.3, **more)
+    attend(hip, store, [400, 99], [90, 3], 4, scale=0.0, **more)
+    attend(hip, store, [400, 120], [90, 120], 4, sharp=60.0, **more)
+
+    def share(tables):
+        tables[1, :10] = tables[0, :10]
+
+    attend(hip, store, [200, 175], [70, 90], 4, spoil=share, **more)
+    store = Store(hip, "int8", 16, 60, 2, rng)
+    for i in (0, 1):
+        for factor in (0.0, 1e-12, 30.0 if i == 0 else 1e9):
+            store.scales[i][rng.random((60, 2)) < 0.15] *= np.float32(factor)
+        store.codes[i][store.scales[i] == 0] = 0
+    attend(hip, store, [400, 120], [90, 120], 4, **more)
+    store = Store(hip, "e4m3", 32, 30, 2, rng)
+
+    def lose(tables):
+        tables[0, 1], tables[0, 3] = -1, 30
+        tables[1, :] = 1 << 30
+        tables[2, 0] = -1
+
+    got = attend(hip, store, [200, 64, 70], [100, 40, 70], 4, spoil=lose, **more)
+    assert np.all(got[100:140] == 0)
+
+
+@pytest.mark.parametrize("kind", BLOCKS)
+def test_attention_in_place_in_blocks(hip, kind):
+    rng = np.random.default_rng(20)
+    store = Store(hip, "int8", 16, 40, 2, rng)
+    rows = 600 + in_blocks(kind, 4)["tail_rows"]
+    q = gen.bf16(rng.standard_normal((rows, 4 * D)).astype(np.float32))
+    tables = dev(hip, np.tile(np.arange(40, dtype=np.int32), (3, 1)))
+    keep = [dev(hip, np.array([600, 0, 9], np.int32)), dev(hip, np.array([0, 590, 590, 599], np.int32))]
+    outs = []
+    for same in (False, True):
+        query = dev(hip, q)
+        out = query if same else dev(hip, q)
+        scratch = hip.DeviceArray(1 << 22, np.uint8)
+        hip.kv8_attention(store.cache, query, out, 4, rows, 3, tables, 40, keep[0], keep[1], max_rows=590,
+                          max_length=4096, workspace=scratch, workspace_bytes=1 << 22)
+        hip.synchronize()
+        outs.append(out.numpy())
+    assert np.array_equal(outs[0], outs[1]) and np.array_equal(outs[0][599:], q[599:])
+    assert not np.array_equal(outs[0][:599], q[:599])
 
 
 def test_attention_far_pages(hip):
