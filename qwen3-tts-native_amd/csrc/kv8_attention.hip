@@ -97,7 +97,7 @@ __device__ __forceinline__ float of_lane(float v, int lane) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: up to 16 (row, head) pairs of one key/value head are the columns
+// Few rows: a tile of up to 16 (row, head) pairs of one key/value head is the columns
 // of 16x16x32 products, keys and values are read once for all of them.  Nothing
 // goes through LDS before the end: a lane's 16 bytes of keys are two operands'
 // rows, its scores' four tokens are those of its four bytes of each dimension.
@@ -107,6 +107,8 @@ __device__ __forceinline__ float of_lane(float v, int lane) {
 // int8, 16 / 8 heads: 446 us, 5.5 TB/s; 64 of 33..4096, e4m3: 60 us, 4.5 TB/s, the
 // longest ones' tail; one of 65521: 33 us, 4.1 TB/s), below by the chain
 // table -> bytes -> products (eight of 97..1024 tokens: 9 us with the join).
+// Rows of short prompts, and some rows over a long context, are tiles in
+// workgroups of their own (one prompt of 801: 20 us; 32 over 16000 tokens: 28).
 // ---------------------------------------------------------------------------
 constexpr int kStep = 64;  // tokens of a wave's step
 constexpr int kStepGranules = kStep / kKv8Granule;
@@ -388,7 +390,7 @@ __global__ __launch_bounds__(32 * kJoinGroups) void kv8_join_kernel(Params p) {
 // Waves are kColumnWaves x kKeyWaves: those of a key group take the same 64 of
 // every 64 * kKeyWaves tokens, and the groups' results are joined at the end.
 // Prompts of 1777..4096 rows, 32 / 8 heads: 361 us, 850 TFLOP/s (the library's
-// large product reaches 1213); one of 801 rows, 16 / 8 heads: 22 us, latency.
+// large product reaches 1213); one of 1024 rows, 16 / 8 heads: 24 us, latency.
 // Two waves a SIMD share the matrix cores (40 % of a busy CU's time), the vector
 // unit (52 %) and LDS (40 %), none of them full: leaving out the exponentials, the
 // value products, the staging or the loads saves 6 to 12 % each.

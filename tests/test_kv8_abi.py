@@ -136,3 +136,22 @@ def test_model_layout_is_one_to_one(is_key):
     raw = model.pack(codes, is_key)
     assert sorted(model._offsets(is_key).ravel()) == list(range(2048))
     assert np.array_equal(model.unpack(raw, is_key), codes)
+
+
+def test_attention_workspace_is_bounded(hip):
+    """Any sizes that a caller may name: an answer, and no more than a small part of the card's memory."""
+    import random
+    draw = random.Random(1)
+
+    def size(bits):
+        return round(2 ** draw.uniform(0, bits))
+
+    for _ in range(20000):
+        heads = draw.choice([1, 2, 4, 8, 16, 32])
+        pages = hip.Kv8Cache("int8", 16, 100, heads, FAKE, FAKE, FAKE, FAKE)
+        rows = size(20)
+        bytes_ = hip.kv8_attention_workspace(pages, heads * draw.choice([1, 2, 3, 5, 8, 16]), rows, size(16) - 1,
+                                             window=draw.choice([0, 0, size(20), 2 ** 31 - 1]),
+                                             max_rows=draw.choice([1, size(12), rows, 2 ** 31 - 1]),
+                                             max_length=draw.choice([size(20), 2 ** 31 - 1]))
+        assert 0 <= bytes_ <= 1 << 28
