@@ -26,6 +26,8 @@ constexpr int kMaxGroup = 16;  // query heads of a key/value head: the columns o
 constexpr float kLog2E = 1.44269504088896340736f;
 
 constexpr int kFewWaves = 4;
+constexpr int kStep = 64;  // tokens of a step of its waves
+constexpr int kMostSplits = 64;
 // Workgroups for sequences of many rows: column waves x key groups of 4 x 1, 4 x 2, 2 x 4.
 enum Many : int { kNone = 0, kWide, kHalved, kQuartered };
 
@@ -35,11 +37,12 @@ struct Params {
     int group = 1;     // query heads of a key/value head
     float scale2 = 0;  // |scale| * log2(e)
     unsigned flip = 0;  // sign bits of a pair of bf16: the query's are flipped for a negative scale
-    int splits = 1;    // workgroups that share a context of few rows
+    int splits = 1;    // workgroups that share a context of few rows, where it has few_tiles tiles
     int columns = 16;  // (row, head of the group) pairs that a shared context can have
     int waves = kFewWaves;  // of a workgroup of few rows
     int many = kNone;
     int few = INT_MAX;  // pairs up to which a sequence counts as one of few rows
+    int few_rows = 0, shared_rows = 0, tile_rows = 0;  // rows of `few`, `columns` and 16 pairs
     int few_tiles = 1;  // workgroups among which the tiles of its rows are dealt
     float* partial_out = nullptr;   // [sequence][kv head][column][split][128]
     float2* partial_sums = nullptr;  // [sequence][kv head][column][split] (maximum, sum)
@@ -62,15 +65,32 @@ __device__ __forceinline__ Rows rows_of(const Params& p, int sequence) {
     return r;
 }
 
-// Workgroups that share the context of a sequence of few rows: 0 where it is
-// not one, 1 where its results do not fit the partial ones' place (more rows
-// than the caller said).
-__device__ __forceinline__ int splits_of(const Params& p, const Rows& r) {
-    if (r.count <= 0 || r.count > p.few / p.group) return 0;
-    return r.count <= p.columns / p.group ? p.splits : 1;
+// a / b for 0 <= a < 2^20, b > 0: the reciprocal's error times a / b is far below the
+// 0.5 / b to the next whole number.  Integer divisions' chains cost 0.4 us a call.
+__device__ __forceinline__ int quotient(int a, int b) {
+    return static_cast<int>((static_cast<float>(a) + 0.5f) * __builtin_amdgcn_rcpf(static_cast<float>(b)));
 }
-__device__ __forceinline__ size_t partial_slot(const Params& p, int sequence, int kv_head, int column) {
-    return ((static_cast<size_t>(sequence) * p.cache.key_value_heads + kv_head) * p.columns + column) * p.splits;
+// How a sequence of few rows is dealt to its workgroups: `tiles` of them take its
+// tiles in turn, `splits` of those share their context.  No splits where it is none
+// of few rows, one where its results do not fit the partial ones' place (more
+// rows than the caller said).  A sequence of fewer tiles than the largest leaves
+// workgroups over: they take shares, of a step of every wave at least (a token
+// over 4000 where 256 rows may come 39 us without, 10.8 with; four sequences 59 / 22).
+struct Shares {
+    int tiles, splits;
+};
+__device__ __forceinline__ Shares shares_of(const Params& p, const Rows& r) {
+    if (r.count <= 0 || r.count > p.few_rows) return Shares{1, 0};
+    if (r.count > p.shared_rows) return Shares{p.few_tiles, 1};
+    if (p.few_tiles == 1 || p.splits == 1) return Shares{p.few_tiles, p.splits};
+    const int tiles = quotient(r.count + p.tile_rows - 1, p.tile_rows);
+    const int reach = p.a.window > 0 ? static_cast<int>(min(static_cast<long long>(p.a.window) + r.count, static_cast<long long>(r.length))) : r.length;
+    const int steps = (reach + kFewWaves * kStep - 1ll) / (kFewWaves * kStep);
+    return Shares{tiles, max(1, min(min(quotient(p.splits * p.few_tiles, tiles), kMostSplits), steps))};
+}
+// A split's place among a column's is its number; columns are `splits` apart.
+__device__ __forceinline__ size_t partial_slot(const Params& p, int sequence, int kv_head, int column, int splits) {
+    return (static_cast<size_t>(sequence) * p.cache.key_value_heads + kv_head) * p.columns * p.splits + static_cast<size_t>(column) * splits;
 }
 
 // Pages and scales of a wave's next 64 granules, one a lane, so that no step
@@ -110,7 +130,6 @@ __device__ __forceinline__ float of_lane(float v, int lane) {
 // Rows of short prompts, and some rows over a long context, are tiles in
 // workgroups of their own (one prompt of 801: 20 us; 32 over 16000 tokens: 28).
 // ---------------------------------------------------------------------------
-constexpr int kStep = 64;  // tokens of a wave's step
 constexpr int kStepGranules = kStep / kKv8Granule;
 
 template <int kWaves>
@@ -129,11 +148,11 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
     const int column = lane & 15, quad = lane >> 4;
     const int kv_head = blockIdx.x, sequence = blockIdx.z;
     const Rows rows = rows_of(p, sequence);
-    const int splits = splits_of(p, rows);
-    const int split = share / p.few_tiles;
-    const int first_tile = p.few_tiles - 1 - share % p.few_tiles;  // a prompt's longest first
+    const auto [tiles, splits] = shares_of(p, rows);
+    const int split = quotient(share, tiles);
+    const int first_tile = tiles - 1 - (share - split * tiles);  // a prompt's longest first
     if (split >= splits) return;
-    const int rows_per_tile = 16 / p.group;
+    const int rows_per_tile = p.tile_rows;
     const int head = kv_head * p.group + column % p.group;
     const int* table = p.a.tables + static_cast<size_t>(sequence) * p.a.table_stride;
     const size_t page_bytes = static_cast<size_t>(p.cache.key_value_heads) * (kPageGranules * kKv8GranuleBytes);
@@ -142,7 +161,7 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
     const unsigned char* keys_of_lane = p.cache.key_pages + kv_head * (kPageGranules * kKv8GranuleBytes) +
                                         (lane & 15) * 64 + quad * 16;
 
-    for (int tile = first_tile * rows_per_tile; tile < rows.count; tile += p.few_tiles * rows_per_tile) {
+    for (int tile = first_tile * rows_per_tile; tile < rows.count; tile += tiles * rows_per_tile) {
         const int row = tile + column / p.group;
         const bool mine = column < rows_per_tile * p.group && row < rows.count;
         const int position = mine ? rows.position + row : -1;
@@ -305,7 +324,7 @@ __device__ __forceinline__ void few_rows(const Params& p, FewShared<kWaves>& lds
         __syncthreads();
         // wave w: dimension tiles of 16, every column
         if (mine) {
-            const size_t slot = partial_slot(p, sequence, kv_head, tile * p.group + column) + split;
+            const size_t slot = partial_slot(p, sequence, kv_head, tile * p.group + column, splits) + split;
 #pragma unroll
             for (int j = 0; j < 8 / kWaves; ++j) {
                 const int d = 8 / kWaves * wave + j;
@@ -344,9 +363,9 @@ __global__ __launch_bounds__(32 * kJoinGroups) void kv8_join_kernel(Params p) {
     const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
     const int column = blockIdx.x, kv_head = blockIdx.y, sequence = blockIdx.z;
     const Rows rows = rows_of(p, sequence);
-    const int splits = splits_of(p, rows);
+    const int splits = shares_of(p, rows).splits;
     if (splits <= 1 || column >= rows.count * p.group) return;
-    const size_t slot = partial_slot(p, sequence, kv_head, column);
+    const size_t slot = partial_slot(p, sequence, kv_head, column, splits);
     float top = -INFINITY, total = 0.0f;
     floatx4_t o{0.f, 0.f, 0.f, 0.f};
     for (int i = group; i < splits; i += kJoinGroups) {
@@ -444,7 +463,7 @@ __device__ __forceinline__ void many_rows(const Params& p, unsigned char* dynami
     const int column = lane & 31, half = lane >> 5;
     const int kv_head = blockIdx.x, sequence = blockIdx.z;
     const Rows rows = rows_of(p, sequence);
-    if (rows.count <= 0 || splits_of(p, rows) > 0) return;
+    if (rows.count <= 0 || shares_of(p, rows).splits > 0) return;
     const int* table = p.a.tables + static_cast<size_t>(sequence) * p.a.table_stride;
     const size_t page_bytes = static_cast<size_t>(p.cache.key_value_heads) * (kPageGranules * kKv8GranuleBytes);
     const unsigned char* keys = p.cache.key_pages + kv_head * (kPageGranules * kKv8GranuleBytes) + lane * 16;
@@ -835,7 +854,7 @@ Dealt dealt_of(const Kv8Cache& cache, const Kv8AttentionArgs& a, size_t workspac
     // 113 / 57.  Not where most sequences would find no tile of theirs.
     const bool tiles_win = few_tiles * (tokens_of(tile) + 120) / 33000 < 4.5 + std::max(0.0116 * chain, 8e-5 * many_blocks * tokens_of(128 / group));
     if (pairs <= 16 || (tiles_win && blocks * tiles_of(pairs) <= 4 * few_tiles + 1024)) {
-        d.columns = static_cast<int>(pairs);
+        d.columns = pairs <= 16 ? static_cast<int>(pairs) : tiles_of(pairs) * tile * group;
     } else {
         // Blocks of 128 columns where that makes one a CU, or where a chain of
         // steps is short anyway; else the tokens of a step are dealt to two or
@@ -861,9 +880,12 @@ Dealt dealt_of(const Kv8Cache& cache, const Kv8AttentionArgs& a, size_t workspac
     const long long there = d.many == kNone ? std::min(blocks * d.few_tiles, few_tiles) : blocks;
     const auto for_blocks = [&](long long n) { return (n + there - 1) / there; };
     const auto for_tokens = [&](int n) { return (static_cast<long long>(reach) + n - 1) / n; };
-    const long long wanted = std::max(for_blocks(256), std::min(for_blocks(512), for_tokens(4096)));
+    long long wanted = std::max(for_blocks(256), std::min(for_blocks(512), for_tokens(4096)));
+    // Where tiles fill the chip by the caller's sizes, a step of few of them still
+    // finds shares (not where the second launch costs more: forty's 16 rows 57, with it 71).
+    if (d.many == kNone && d.few_tiles > 1 && there <= 512) wanted = std::max(wanted, std::min(2LL, for_tokens(1024)));
     const long long fits = static_cast<long long>(workspace_bytes / (static_cast<size_t>(blocks) * d.columns * kBytesOfPartial));
-    d.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({wanted, for_tokens(kFewWaves * kStep), fits, 64, 65535 / d.few_tiles})));
+    d.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({wanted, for_tokens(kFewWaves * kStep), fits, kMostSplits, 65535 / d.few_tiles})));
     // Short contexts of many sequences: a wave a workgroup, none waits at the
     // end for waves that had no step (256 sequences of 100 tokens 24.9 us, now
     // 15.7; of 1111..8192 tokens 445, a wave each 499).
@@ -912,6 +934,9 @@ hipError_t launch_kv8_attention(const Kv8Cache& cache, const Kv8AttentionArgs& a
     p.many = d.many;
     p.few = d.few;
     p.few_tiles = d.few_tiles;
+    p.few_rows = d.few / p.group;
+    p.shared_rows = d.columns / p.group;
+    p.tile_rows = 16 / p.group;
     const size_t slots = static_cast<size_t>(a.sequences) * cache.key_value_heads * d.columns * d.splits;
     p.partial_out = a.workspace;
     p.partial_sums = reinterpret_cast<float2*>(a.workspace + slots * kDim);

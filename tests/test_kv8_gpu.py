@@ -609,6 +609,17 @@ def test_attention_long_context_of_some_rows(hip, workspace, new, kind):
     attend(hip, store, [5000, 900, 64], new, 2, workspace=workspace, **more)
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 1), (7, 1), (16, 1), (2, 2)])
+@pytest.mark.parametrize("new", [[1, 1, 1, 0], [1, 17, 3, 1], [40, 1, 9, 16], [60, 60, 2, 30]])
+@pytest.mark.parametrize("workspace", [1 << 14, 1 << 25])
+@pytest.mark.parametrize("window", [0, 700])
+def test_attention_of_fewer_rows_than_named(hip, heads, kv_heads, new, workspace, window):
+    """A captured step's sizes, of which each sequence uses some: what is left over shares the contexts."""
+    rng = np.random.default_rng(heads)
+    store = Store(hip, "int8", 32, 230, kv_heads, rng)
+    attend(hip, store, [5000, 900, 300, 257], new, heads, window=window, workspace=workspace, max_rows=60, tail_rows=100)
+
+
 @pytest.mark.parametrize("kind", BLOCKS)
 def test_attention_of_odd_numbers_in_blocks(hip, kind):
     """Strides, scales, scores far apart, pages of unequal scales, tables that share pages or name none."""
